@@ -742,6 +742,172 @@ int omni_channel_embedding_sum(const void* token_ids, int ids_dtype, int64_t row
                                const uint64_t* tables, const int64_t* vocab_sizes, int dtype,
                                int64_t hidden, void* out, omni_stream_t stream);
 
+/*
+ * Linear layers in 8-bit floating point (OCP E4M3) with a float32 scale for each block of 128.
+ *
+ * omni_block_quantize: rows of bf16 / f16 / f32 values to such rows. Each group of 128 values of a
+ * row (the last one shorter) takes scale = amax / 448 and q = E4M3(x * (448 / amax)), both in
+ * float32, rounded to nearest even; a group whose largest magnitude is below 2^-100 holds zeros
+ * with scale 1. NaN stays NaN; a group with an infinity has an infinite scale, so that every
+ * product with it is NaN. x rows x_stride elements apart; q rows q_stride bytes apart (a multiple
+ * of 16, q 16-byte aligned) with k rounded up to 16 values each, the added ones zero; scale
+ * [rows][ceil(k / 128)], rows scale_stride apart. rows = 0 does nothing.
+ */
+int omni_block_quantize(const void* x, int x_dtype, int64_t x_stride, int64_t rows, int64_t k,
+                        void* q, int64_t q_stride, float* scale, int64_t scale_stride,
+                        omni_stream_t stream);
+
+/*
+ * omni_block_fp8_gemm: out[m][n] = sum_b x_scale[m][b] * w_scale[n / 128][b] *
+ * sum_{k in block b} x[m][k] * w[n][k] (+ bias[n]), float32 sums, rounded once to out_dtype
+ * (bf16, f16 or f32). x [rows][k] and w [n][k] E4M3, 16-byte aligned, rows x_stride / w_stride
+ * bytes apart (multiples of 16), k a multiple of 16 up to 2^20; x_scale at m * x_scale_stride_row
+ * + b * x_scale_stride_block; w_scale rows w_scale_stride apart. out rows out_stride elements
+ * apart, any alignment of its type, and no input. rows = 0 does nothing.
+ */
+typedef struct omni_block_fp8_args {
+  const void* x;
+  int64_t x_stride;
+  const float* x_scale;
+  int64_t x_scale_stride_row, x_scale_stride_block;
+  const void* w;
+  int64_t w_stride;
+  const float* w_scale;
+  int64_t w_scale_stride;
+  int64_t rows, n, k;
+  const float* bias;
+  void* out;
+  int64_t out_stride;
+  int out_dtype;
+} omni_block_fp8_args;
+int omni_block_fp8_gemm(const omni_block_fp8_args* args, omni_stream_t stream);
+
+/*
+ * omni_gated_residual_norm: the step between two blocks of a transformer,
+ *
+ *   u = post_norm ? norm(y) * post_weight + post_bias : y
+ *   residual = x + scale * act(gate) * u           rounded to x's type
+ *   normed = norm(x + scale * act(gate) * u) * pre_weight + pre_bias     (before that rounding)
+ *
+ * norm RMS: v / sqrt(mean(v^2) + eps); LAYER: (v - mean) / sqrt(mean((v - mean)^2) + eps).
+ * Weights and biases float32 [channels], each optional (biases with LAYER only). gate optional:
+ * row r reads gate row r / rows_per_gate. All arithmetic in float32. y bf16 / f16 / f32, x of
+ * y's type or float32; normed bf16 / f16 / f32, or E4M3 with a scale per group of 128 as
+ * omni_block_quantize makes them from the float32 values (normed 16-byte aligned, its stride a
+ * multiple of 16). Row strides in elements; any alignment of the type otherwise. residual may be
+ * x, normed may be y of the same type and stride. channels up to 32768 (else
+ * OMNI_ERR_UNSUPPORTED); rows = 0 does nothing.
+ */
+enum { OMNI_NORM_RMS = 0, OMNI_NORM_LAYER = 1 };
+enum { OMNI_GATE_NONE = 0, OMNI_GATE_SIGMOID = 1, OMNI_GATE_TANH = 2 };
+typedef struct omni_gated_norm_args {
+  const void* x;
+  int x_dtype;
+  int64_t x_stride;
+  const void* y;
+  int y_dtype;
+  int64_t y_stride;
+  int64_t rows, channels;
+  int norm;
+  int post_norm;
+  float eps, scale;
+  const float* post_weight;
+  const float* post_bias;
+  const float* pre_weight;
+  const float* pre_bias;
+  const void* gate;
+  int gate_dtype;
+  int64_t gate_stride, rows_per_gate;
+  int gate_activation;
+  void* residual;
+  int64_t residual_stride;
+  void* normed;
+  int normed_dtype;
+  int64_t normed_stride;
+  float* normed_scale;
+  int64_t normed_scale_stride;
+} omni_gated_norm_args;
+int omni_gated_residual_norm(const omni_gated_norm_args* args, omni_stream_t stream);
+
+/*
+ * omni_rotary: rotary positions of q [tokens][heads][dim] and k [tokens][kv_heads][dim] (k absent
+ * with kv_heads = 0), of one type (bf16, f16, f32), token and head strides free, dim contiguous.
+ * The first 2 * pairs values of a head are turned, the rest copied: pair i of token t becomes
+ * (a cos - b sin, b cos + a sin) * factor with angle positions[t] * inv_freq[i], computed in
+ * float64 (inv_freq float64 [pairs]); pairs (i, i + pairs) in the HALF layout, (2 i, 2 i + 1)
+ * INTERLEAVED. transposed turns by the negative angle (the gradient of the forward form).
+ * positions int32 or int64, any sign. Outputs may be the inputs (same strides), else overlap
+ * nothing. tokens = 0 does nothing.
+ */
+enum { OMNI_ROTARY_HALF = 0, OMNI_ROTARY_INTERLEAVED = 1 };
+typedef struct omni_rotary_args {
+  const void* q;
+  int64_t q_stride_token, q_stride_head;
+  const void* k;
+  int64_t k_stride_token, k_stride_head;
+  void* q_out;
+  int64_t q_out_stride_token, q_out_stride_head;
+  void* k_out;
+  int64_t k_out_stride_token, k_out_stride_head;
+  int dtype;
+  int64_t tokens, heads, kv_heads, dim, pairs;
+  const void* positions;
+  int positions_dtype;
+  int64_t positions_stride;
+  const double* inv_freq;
+  float factor;
+  int layout;
+  int transposed;
+} omni_rotary_args;
+int omni_rotary(const omni_rotary_args* args, omni_stream_t stream);
+
+/*
+ * omni_adjust_logits: what a sampler does to logits [rows][vocab] (f32, bf16, f16) before it draws,
+ * in this order, in float32, rounded once to out_dtype (dtype or f32):
+ *
+ *   tokens of the row's history          l = l > 0 ? l / repetition[row] : l * repetition[row]
+ *   those past its prompt, count times   l -= frequency[row] * count + presence[row]
+ *   the row's bias list                  l += bias_values[row][i] for token bias_tokens[row][i];
+ *                                        of several entries for one token the last stands
+ *   the row's mask                       l = -infinity where the token's bit is 0
+ *
+ * Each part is optional. history [slots][capacity] int32 / int64 token ids (tokens_dtype, as
+ * bias_tokens), rows history_stride apart; row r reads slot slot_index[r] (or r), its first
+ * lengths[slot] tokens (clamped to capacity), of which the first prompt_lengths[slot] are the
+ * prompt; a slot out of range has no history. Ids outside [0, vocab) are passed over. allowed
+ * [masks][ceil(vocab / 32)] int32, token v at bit v % 32 of word v / 32, rows allowed_stride
+ * apart; row r reads mask allowed_index[r] (or r), none where that is out of range. A row whose
+ * mask allows nothing is all -infinity. out may be logits (same type and stride). vocab up to
+ * 2^30; rows = 0 does nothing.
+ */
+typedef struct omni_logits_args {
+  const void* logits;
+  int dtype;
+  int64_t logits_stride;
+  void* out;
+  int out_dtype;
+  int64_t out_stride;
+  int64_t rows, vocab;
+  const void* history;
+  int tokens_dtype;
+  int64_t history_stride, capacity, slots;
+  const void* lengths;
+  const void* prompt_lengths;
+  int lengths_dtype;
+  const int64_t* slot_index;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const void* bias_tokens;
+  int64_t bias_tokens_stride;
+  const float* bias_values;
+  int64_t bias_values_stride, biases;
+  const int32_t* allowed;
+  int64_t allowed_stride, masks;
+  const int64_t* allowed_index;
+} omni_logits_args;
+int omni_adjust_logits(const omni_logits_args* args, omni_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

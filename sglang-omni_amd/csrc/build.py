@@ -32,7 +32,8 @@ SOURCES = ["capi.hip", "rvq.hip", "conv.hip", "conv_k7_raw_wbf16.hip", "conv_k7_
            "residual_stack_wfp8.hip", "single_output_conv.hip", "codec_state.hip", "snake.hip", "hift.hip",
            "egress.hip", "code2wav_front.hip", "channel_embedding.hip", "conv_general.hip",
            "conv_general_f32.hip", "conv_general_bf16.hip", "conv_general_f16.hip",
-           "gemm.hip", "resblock_pair.hip"]
+           "gemm.hip", "resblock_pair.hip", "block_fp8.hip", "gated_norm.hip", "rotary.hip",
+           "logits.hip"]
 
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -195,7 +195,136 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class BlockFp8Args(ctypes.Structure):
+    """Mirror of ``omni_block_fp8_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("x_scale", ctypes.c_void_p),
+        ("x_scale_stride_row", ctypes.c_int64),
+        ("x_scale_stride_block", ctypes.c_int64),
+        ("w", ctypes.c_void_p),
+        ("w_stride", ctypes.c_int64),
+        ("w_scale", ctypes.c_void_p),
+        ("w_scale_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("out_dtype", ctypes.c_int),
+    ]
+
+
+class GatedNormArgs(ctypes.Structure):
+    """Mirror of ``omni_gated_norm_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_dtype", ctypes.c_int),
+        ("x_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_dtype", ctypes.c_int),
+        ("y_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("norm", ctypes.c_int),
+        ("post_norm", ctypes.c_int),
+        ("eps", ctypes.c_float),
+        ("scale", ctypes.c_float),
+        ("post_weight", ctypes.c_void_p),
+        ("post_bias", ctypes.c_void_p),
+        ("pre_weight", ctypes.c_void_p),
+        ("pre_bias", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("gate_dtype", ctypes.c_int),
+        ("gate_stride", ctypes.c_int64),
+        ("rows_per_gate", ctypes.c_int64),
+        ("gate_activation", ctypes.c_int),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("normed", ctypes.c_void_p),
+        ("normed_dtype", ctypes.c_int),
+        ("normed_stride", ctypes.c_int64),
+        ("normed_scale", ctypes.c_void_p),
+        ("normed_scale_stride", ctypes.c_int64),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``omni_rotary_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_stride_token", ctypes.c_int64),
+        ("q_out_stride_head", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p),
+        ("k_out_stride_token", ctypes.c_int64),
+        ("k_out_stride_head", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+        ("pairs", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("positions_dtype", ctypes.c_int),
+        ("positions_stride", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p),
+        ("factor", ctypes.c_float),
+        ("layout", ctypes.c_int),
+        ("transposed", ctypes.c_int),
+    ]
+
+
+class LogitsArgs(ctypes.Structure):
+    """Mirror of ``omni_logits_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("logits_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_dtype", ctypes.c_int),
+        ("out_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("history", ctypes.c_void_p),
+        ("tokens_dtype", ctypes.c_int),
+        ("history_stride", ctypes.c_int64),
+        ("capacity", ctypes.c_int64),
+        ("slots", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("prompt_lengths", ctypes.c_void_p),
+        ("lengths_dtype", ctypes.c_int),
+        ("slot_index", ctypes.c_void_p),
+        ("repetition", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p),
+        ("bias_tokens", ctypes.c_void_p),
+        ("bias_tokens_stride", ctypes.c_int64),
+        ("bias_values", ctypes.c_void_p),
+        ("bias_values_stride", ctypes.c_int64),
+        ("biases", ctypes.c_int64),
+        ("allowed", ctypes.c_void_p),
+        ("allowed_stride", ctypes.c_int64),
+        ("masks", ctypes.c_int64),
+        ("allowed_index", ctypes.c_void_p),
+    ]
+
+
 GEMM_STORE, GEMM_SILU_MUL, GEMM_GELU, GEMM_SCALED_RESIDUAL = 0, 1, 2, 3
+NORM_RMS, NORM_LAYER = 0, 1
+GATE_NONE, GATE_SIGMOID, GATE_TANH = 0, 1, 2
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -261,6 +390,11 @@ SIGNATURES: dict[str, list] = {
     "omni_resblock_pair": [ctypes.POINTER(ConvArgs), ctypes.POINTER(ConvArgs), _PTR],
     "omni_channel_embedding_sum": [_PTR, _INT, _I64, _I64, _I64, _I64, _PTR, _PTR, _INT, _I64, _PTR,
                                    _PTR],
+    "omni_block_quantize": [_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _PTR, _I64, _PTR],
+    "omni_block_fp8_gemm": [ctypes.POINTER(BlockFp8Args), _PTR],
+    "omni_gated_residual_norm": [ctypes.POINTER(GatedNormArgs), _PTR],
+    "omni_rotary": [ctypes.POINTER(RotaryArgs), _PTR],
+    "omni_adjust_logits": [ctypes.POINTER(LogitsArgs), _PTR],
 }
 _RESTYPES = {"omni_codec_error_string": ctypes.c_char_p}
 
@@ -353,6 +487,11 @@ def stream_handle(device: torch.device | None = None) -> int:
             and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """The stride between a matrix's rows: its width where one row's stride says nothing."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
