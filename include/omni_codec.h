@@ -764,10 +764,21 @@ int omni_block_quantize(const void* x, int x_dtype, int64_t x_stride, int64_t ro
  * bytes apart (multiples of 16), k a multiple of 16 up to 2^20; x_scale at m * x_scale_stride_row
  * + b * x_scale_stride_block; w_scale rows w_scale_stride apart. out rows out_stride elements
  * apart, any alignment of its type, and no input. rows = 0 does nothing.
+ *
+ * x may be bf16 / f16 / f32 rows instead (x_dtype, x_stride in elements, any alignment of the type;
+ * `features` of them, which rounded up to 16 make k): they are quantized as omni_block_quantize
+ * does, up to OMNI_BLOCK_FP8_FEW_ROWS rows inside the product's launch, more of them in a launch
+ * before it into workspace (16-byte aligned, at least rows * (k + 4 * ceil(k / 128)) bytes).
+ *
+ * bf16 outputs multiply on the 8-bit matrix cores, which cut each product below 2^-13 of the
+ * largest of the 8 it is added with (up to 5e-5 of a result); f16 and f32 outputs on the bf16 ones,
+ * where the sums are float32 throughout.
  */
+enum { OMNI_BLOCK_FP8_FEW_ROWS = 16 };
 typedef struct omni_block_fp8_args {
   const void* x;
-  int64_t x_stride;
+  int x_dtype;
+  int64_t x_stride, features;
   const float* x_scale;
   int64_t x_scale_stride_row, x_scale_stride_block;
   const void* w;
@@ -779,6 +790,8 @@ typedef struct omni_block_fp8_args {
   void* out;
   int64_t out_stride;
   int out_dtype;
+  void* workspace;
+  int64_t workspace_bytes;
 } omni_block_fp8_args;
 int omni_block_fp8_gemm(const omni_block_fp8_args* args, omni_stream_t stream);
 

@@ -49,16 +49,24 @@ OMNI_DEVICE void store_values(T* dst, int64_t valid, const float (&v)[N]) {
   }
 }
 
+// A group's scale from its largest magnitude, and the factor its values take. NaN stays NaN through
+// them; an infinity makes the scale infinite, so the group's products are NaN.
+OMNI_DEVICE float group_scale(float amax, float* unit) {
+  const bool tiny = amax < kTinyGroup;
+  *unit = tiny ? 1.f : kE4m3Max / amax;
+  return tiny ? 1.f : amax / kE4m3Max;
+}
+
 // 8 values of a group of 128 held by 16 consecutive lanes, 8 each: their E4M3 bytes and the group's
-// scale. NaN stays NaN; an infinity makes the scale infinite, so the group's products are NaN.
+// scale.
 OMNI_DEVICE float quantize_group(const float (&v)[8], u32x2* packed) {
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
 #pragma unroll
   for (int off = 1; off < 16; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 16));
-  const bool tiny = amax < kTinyGroup;
-  const float unit = tiny ? 1.f : kE4m3Max / amax;
+  float unit;
+  const float scale = group_scale(amax, &unit);
   u32x2 p = {0u, 0u};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -66,7 +74,7 @@ OMNI_DEVICE float quantize_group(const float (&v)[8], u32x2* packed) {
     p[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * unit, v[4 * h + 3] * unit, p[h], true);
   }
   *packed = p;
-  return tiny ? 1.f : amax / kE4m3Max;
+  return scale;
 }
 
 OMNI_DEVICE i32x8 read_operand(const uint8_t* row, int slot0, int slot1) {
@@ -117,24 +125,4 @@ OMNI_DEVICE f32x4 block_product(const Operand<true>& a, const Operand<true>& b) 
 #pragma unroll
   for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[s], b.v[s], c, 0, 0, 0);
   return c;
-}
-
-// Four consecutive columns of one row, rounded once to the output's type.
-OMNI_DEVICE void store_columns(void* out, int dtype, int64_t stride, const float* bias,
-                               int64_t row, int64_t rows, int64_t col, int64_t n, f32x4 v) {
-  if (row >= rows || col >= n) return;
-  const int64_t valid = n - col;
-  if (bias) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < valid) v[e] += bias[col + e];
-  }
-  const float o[4] = {v[0], v[1], v[2], v[3]};
-  const int64_t at = row * stride + col;
-  if (dtype == OMNI_DTYPE_F32)
-    store_values<float, 4>(static_cast<float*>(out) + at, valid, o);
-  else if (dtype == OMNI_DTYPE_BF16)
-    store_values<__bf16, 4>(static_cast<__bf16*>(out) + at, valid, o);
-  else
-    store_values<_Float16, 4>(static_cast<_Float16*>(out) + at, valid, o);
 }

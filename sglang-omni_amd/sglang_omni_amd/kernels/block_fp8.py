@@ -6,7 +6,6 @@ cores; scales and sums are float32."""
 
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -106,44 +105,72 @@ def block_fp8_linear(x: torch.Tensor | BlockFp8Rows, weight: BlockFp8Weight,
                      out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """out = x @ W^T + bias [rows, out_features] on the current stream, float32 sums rounded once to
     out_dtype (bf16, f16 or f32; ``out``'s own when it is given). x is ``BlockFp8Rows``, or a float
-    tensor [rows, in_features] that is quantized as ``quantize_block_rows`` does."""
-    if not isinstance(x, BlockFp8Rows):
-        x = quantize_block_rows(x)
-    values, scale, w, ws = x.values, x.scale, weight.weight, weight.scale
-    device = values.device
-    N.require_device(values, scale, w, ws, weight.bias, out)
-    if values.dtype != _E4M3 or w.dtype != _E4M3 or values.dim() != 2 or w.dim() != 2:
-        raise ValueError("x and the weight must be float8_e4m3fn matrices")
-    rows, k = values.shape
-    n = w.shape[0]
-    if w.shape[1] != k:
-        raise ValueError(f"x has {k} features, the weight takes {w.shape[1]}")
-    blocks = (k + BLOCK - 1) // BLOCK
-    if (scale.dtype != torch.float32 or scale.shape != (rows, blocks)
-            or ws.dtype != torch.float32 or ws.shape != ((n + BLOCK - 1) // BLOCK, blocks)
-            or (ws.stride(1) != 1 and blocks > 1)):
-        raise ValueError("scales must be float32 [rows, ceil(in / 128)] and "
-                         "[ceil(out / 128), ceil(in / 128)]")
-    if (values.stride(1) != 1 and k > 1) or (w.stride(1) != 1 and k > 1):
-        raise ValueError("x and the weight must have contiguous rows")
-    bias = weight.bias
-    if bias is not None:
-        N.require_vector(bias, n, "bias", device)
-    if out is None:
-        out = torch.empty(rows, n, dtype=out_dtype, device=device)
-    elif out.shape != (rows, n) or (out.stride(1) != 1 and n > 1):
-        raise ValueError(f"out must be [{rows}, {n}] with contiguous rows")
-    if out.dtype not in _FLOATS:
-        raise ValueError("out must be bf16, f16 or f32")
-    if not (device == scale.device == w.device == ws.device == out.device):
+    tensor [rows, features] that is quantized as ``quantize_block_rows`` does. bf16 outputs multiply
+    on the 8-bit matrix cores (up to 5e-5 of a result off); f16 and f32 ones on the bf16 matrix
+    cores, exact products in float32 sums, at about half the rate."""
+    w, w_scale, bias = weight.weight, weight.scale, weight.bias
+    if type(x) is BlockFp8Rows:
+        values, scale = x.values, x.scale
+    else:
+        values, scale = x, None
+    index = values.get_device()
+    if index < 0 or w.get_device() != index or w_scale.get_device() != index \
+            or (scale is not None and scale.get_device() != index) \
+            or (out is not None and out.get_device() != index):
+        N.require_device(values, scale, w, w_scale, out)
         raise ValueError("x, the weight and out must be on one GPU")
-    args = N.BlockFp8Args(values.data_ptr(), N.row_stride(values), scale.data_ptr(),
-                          scale.stride(0), scale.stride(1), w.data_ptr(), N.row_stride(w),
-                          ws.data_ptr(), N.row_stride(ws), rows, n, k, N.ptr(bias),
-                          out.data_ptr(), N.row_stride(out), N.omni_dtype(out.dtype))
-    lib = N.load_library()
-    N.check(lib.omni_block_fp8_gemm(ctypes.byref(args), N.stream_handle(device)),
-            "omni_block_fp8_gemm")
+    if w.dtype is not _E4M3 or w.dim() != 2 or values.dim() != 2:
+        raise ValueError("the weight must be a float8_e4m3fn matrix, x a matrix")
+    rows, features = values.shape
+    n, k = w.shape
+    blocks = (k + BLOCK - 1) // BLOCK
+    x_stride, x_contiguous = values.stride()
+    w_stride, w_contiguous = w.stride()
+    if (x_contiguous != 1 and features > 1) or (w_contiguous != 1 and k > 1):
+        raise ValueError("x and the weight must have contiguous rows")
+    if w_scale.dtype is not torch.float32 or w_scale.shape != ((n + BLOCK - 1) // BLOCK, blocks) \
+            or (blocks > 1 and w_scale.stride(1) != 1):
+        raise ValueError("the weight's scale must be float32 [ceil(out / 128), ceil(in / 128)] with "
+                         "contiguous rows")
+    workspace, workspace_bytes = None, 0
+    if scale is not None:
+        if values.dtype is not _E4M3 or features != k:
+            raise ValueError(f"x must be float8_e4m3fn rows of the weight's {k} features")
+        if scale.dtype is not torch.float32 or scale.shape != (rows, blocks):
+            raise ValueError("x's scale must be float32 [rows, ceil(in / 128)]")
+        scale_ptr = scale.data_ptr()
+        scale_row, scale_block = scale.stride()
+    else:
+        if values.dtype not in _FLOATS:
+            raise ValueError("x must be BlockFp8Rows, or bf16, f16 or f32 rows")
+        if (features + 15) // 16 * 16 != k:
+            raise ValueError(f"x has {features} features, the weight takes {k}")
+        scale_ptr = scale_row = scale_block = 0
+        if rows > N.BLOCK_FP8_FEW_ROWS:
+            workspace_bytes = rows * (k + 4 * blocks)
+            workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=values.device)
+    if bias is not None:
+        N.require_vector(bias, n, "bias", values.device)
+    if out is None:
+        if out_dtype not in _FLOATS:
+            raise ValueError("out must be bf16, f16 or f32")
+        out = torch.empty((rows, n), dtype=out_dtype, device=values.device)
+        out_stride = n
+    else:
+        out_dtype = out.dtype
+        if out.shape != (rows, n) or (n > 1 and out.stride(1) != 1) or out_dtype not in _FLOATS:
+            raise ValueError(f"out must be bf16, f16 or f32 [{rows}, {n}] with contiguous rows")
+        out_stride = N.row_stride(out)
+    codes = N.TORCH_TO_OMNI
+    args = N.pack_block_fp8(
+        values.data_ptr(), codes[values.dtype], x_stride if rows > 1 else features, features,
+        scale_ptr, scale_row, scale_block, w.data_ptr(), w_stride if n > 1 else k,
+        w_scale.data_ptr(), N.row_stride(w_scale), rows, n, k,
+        0 if bias is None else bias.data_ptr(), out.data_ptr(), out_stride, codes[out_dtype],
+        0 if workspace is None else workspace.data_ptr(), workspace_bytes)
+    status = N.load_library().omni_block_fp8_gemm(args, N.raw_stream(index))
+    if status:
+        N.check(status, "omni_block_fp8_gemm")
     return out
 
 

@@ -4,8 +4,6 @@ residual scale, the residual add, and the norm before the next block, optionally
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from .. import _native as N
@@ -14,6 +12,16 @@ from .block_fp8 import BLOCK, BlockFp8Rows
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _NORMS = {"rms": N.NORM_RMS, "layer": N.NORM_LAYER}
 _ACTIVATIONS = {"none": N.GATE_NONE, "sigmoid": N.GATE_SIGMOID, "tanh": N.GATE_TANH}
+
+
+def _vector(t: torch.Tensor | None, channels: int, index: int, what: str) -> int:
+    """The address of a per-channel float32 vector on GPU ``index``, 0 for none."""
+    if t is None:
+        return 0
+    if t.dtype is not torch.float32 or t.shape != (channels,) or t.get_device() != index \
+            or (channels > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what} must be contiguous float32 [{channels}] on x's GPU")
+    return t.data_ptr()
 
 
 def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", eps: float = 1e-6,
@@ -36,71 +44,71 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", 
     gate is [channels], or [G, channels] with rows % G == 0: rows / G consecutive rows share a gate
     (one per sequence; one per token with G = rows). normed has ``normed_dtype`` (y's by default);
     with ``torch.float8_e4m3fn`` it is ``BlockFp8Rows``. ``residual_out`` may be x."""
-    N.require_device(x, y, gate, residual_out)
-    if x.dim() != 2 or x.shape != y.shape or x.stride(1) != 1 and x.shape[1] > 1 \
-            or y.stride(1) != 1 and y.shape[1] > 1:
-        raise ValueError("x and y must be [rows, channels] alike, with contiguous rows")
-    if y.dtype not in _FLOATS or (x.dtype != y.dtype and x.dtype != torch.float32):
+    index = x.get_device()
+    if index < 0 or y.get_device() != index or (gate is not None and gate.get_device() != index):
+        N.require_device(x, y, gate)
+        raise ValueError("x, y and gate must be on one GPU")
+    x_dtype, y_dtype = x.dtype, y.dtype
+    if x.dim() != 2 or x.shape != y.shape:
+        raise ValueError("x and y must be [rows, channels] alike")
+    rows, c = x.shape
+    x_stride, x_contiguous = x.stride()
+    y_stride, y_contiguous = y.stride()
+    if c < 1 or (c > 1 and (x_contiguous != 1 or y_contiguous != 1)):
+        raise ValueError("x and y must have contiguous rows of at least one channel")
+    if y_dtype not in _FLOATS or (x_dtype is not y_dtype and x_dtype is not torch.float32):
         raise ValueError("y must be bf16, f16 or f32, and x of y's dtype or float32")
     if norm not in _NORMS or gate_activation not in _ACTIVATIONS:
         raise ValueError(f"unknown norm {norm!r} or gate activation {gate_activation!r}")
-    rows, c = x.shape
-    device = x.device
-    if c < 1:
-        raise ValueError("x has no channels")
     if norm == "rms" and (post_bias is not None or pre_bias is not None):
         raise ValueError("biases go with the layer norm")
     if not post_norm and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias go with post_norm")
-    if post_weight is not None:
-        N.require_vector(post_weight, c, "post_weight", device)
-    if post_bias is not None:
-        N.require_vector(post_bias, c, "post_bias", device)
-    if pre_weight is not None:
-        N.require_vector(pre_weight, c, "pre_weight", device)
-    if pre_bias is not None:
-        N.require_vector(pre_bias, c, "pre_bias", device)
-    if y.device != device or (gate is not None and gate.device != device):
-        raise ValueError("x, y and gate must be on one GPU")
-    gate_ptr, gate_dtype, gate_stride, rows_per_gate = None, N.DTYPE_F32, 0, 1
+    gate_ptr, gate_code, gate_stride, rows_per_gate = 0, N.DTYPE_F32, 0, 1
     if gate is not None:
-        gates = 1 if gate.dim() == 1 else gate.shape[0]
-        if (gate.dim() not in (1, 2) or gate.shape[-1] != c or gate.dtype not in _FLOATS
-                or (gate.stride(-1) != 1 and c > 1) or gates < 1 or rows % gates):
+        gate_shape = gate.shape
+        gates = gate_shape[0] if len(gate_shape) == 2 else 1
+        if (len(gate_shape) not in (1, 2) or gate_shape[-1] != c or gate.dtype not in _FLOATS
+                or (c > 1 and gate.stride(-1) != 1) or gates < 1 or rows % gates):
             raise ValueError("gate must be bf16, f16 or f32 [channels] or [G, channels], rows a "
                              "multiple of G, with contiguous rows")
-        gate_ptr, gate_dtype = gate.data_ptr(), N.omni_dtype(gate.dtype)
-        # a stride of 0 is a gate expanded over its rows
-        gate_stride = gate.stride(0) if gate.dim() == 2 else 0
+        gate_ptr, gate_code = gate.data_ptr(), N.TORCH_TO_OMNI[gate.dtype]
+        if gates > 1:
+            gate_stride = gate.stride(0)  # 0 for a gate expanded over its rows
         rows_per_gate = max(rows // gates, 1)
     elif gate_activation != "none":
         raise ValueError("gate_activation goes with a gate")
+    device = x.device
     if residual_out is None:
-        residual_out = torch.empty(rows, c, dtype=x.dtype, device=device)
-    elif (residual_out.shape != x.shape or residual_out.dtype != x.dtype
-          or (residual_out.stride(1) != 1 and c > 1) or residual_out.device != device):
-        raise ValueError("residual_out must be like x, with contiguous rows")
-    dtype = y.dtype if normed_dtype is None else normed_dtype
-    normed_scale = None
-    if dtype == torch.float8_e4m3fn:
-        normed = torch.empty(rows, (c + 15) // 16 * 16, dtype=dtype, device=device)
-        normed_scale = torch.empty(rows, (c + BLOCK - 1) // BLOCK, dtype=torch.float32,
-                                   device=device)
-    elif dtype in _FLOATS:
-        normed = torch.empty(rows, c, dtype=dtype, device=device)
+        residual_out = torch.empty((rows, c), dtype=x_dtype, device=device)
+        out_stride = c
     else:
+        if (residual_out.shape != x.shape or residual_out.dtype is not x_dtype
+                or (c > 1 and residual_out.stride(1) != 1) or residual_out.get_device() != index):
+            raise ValueError("residual_out must be like x, with contiguous rows")
+        out_stride = N.row_stride(residual_out)
+    if normed_dtype is None:
+        normed_dtype = y_dtype
+    normed_scale, scale_ptr, scale_stride, normed_width = None, 0, 0, c
+    if normed_dtype is torch.float8_e4m3fn:
+        normed_width, scale_stride = (c + 15) // 16 * 16, (c + BLOCK - 1) // BLOCK
+        normed_scale = torch.empty((rows, scale_stride), dtype=torch.float32, device=device)
+        scale_ptr = normed_scale.data_ptr()
+    elif normed_dtype not in _FLOATS:
         raise ValueError("normed_dtype must be bf16, f16, f32 or float8_e4m3fn")
-    args = N.GatedNormArgs(
-        x.data_ptr(), N.omni_dtype(x.dtype), N.row_stride(x), y.data_ptr(),
-        N.omni_dtype(y.dtype), N.row_stride(y), rows, c, _NORMS[norm],
-        int(post_norm), eps, scale, N.ptr(post_weight), N.ptr(post_bias), N.ptr(pre_weight),
-        N.ptr(pre_bias), gate_ptr, gate_dtype, gate_stride, rows_per_gate,
-        _ACTIVATIONS[gate_activation], residual_out.data_ptr(),
-        N.row_stride(residual_out), normed.data_ptr(), N.omni_dtype(dtype),
-        normed.shape[1], N.ptr(normed_scale), 0 if normed_scale is None else normed_scale.shape[1])
-    lib = N.load_library()
-    N.check(lib.omni_gated_residual_norm(ctypes.byref(args), N.stream_handle(device)),
-            "omni_gated_residual_norm")
+    normed = torch.empty((rows, normed_width), dtype=normed_dtype, device=device)
+    codes = N.TORCH_TO_OMNI
+    args = N.pack_gated_norm(
+        x.data_ptr(), codes[x_dtype], x_stride if rows > 1 else c, y.data_ptr(), codes[y_dtype],
+        y_stride if rows > 1 else c, rows, c, _NORMS[norm], 1 if post_norm else 0, eps, scale,
+        _vector(post_weight, c, index, "post_weight"), _vector(post_bias, c, index, "post_bias"),
+        _vector(pre_weight, c, index, "pre_weight"), _vector(pre_bias, c, index, "pre_bias"),
+        gate_ptr, gate_code, gate_stride, rows_per_gate, _ACTIVATIONS[gate_activation],
+        residual_out.data_ptr(), out_stride, normed.data_ptr(), codes[normed_dtype], normed_width,
+        scale_ptr, scale_stride)
+    status = N.load_library().omni_gated_residual_norm(args, N.raw_stream(index))
+    if status:
+        N.check(status, "omni_gated_residual_norm")
     return residual_out, normed if normed_scale is None else BlockFp8Rows(normed, normed_scale)
 
 

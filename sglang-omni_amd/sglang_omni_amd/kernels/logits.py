@@ -3,8 +3,6 @@ of a row's history, its bias list, and its grammar's mask."""
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from .. import _native as N
@@ -13,28 +11,25 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int32, torch.int64)
 
 
-def _per_row(t: torch.Tensor | None, rows: int, what: str, device: torch.device) -> int | None:
+def _per_row(t: torch.Tensor | None, rows: int, dtype: torch.dtype, what: str, index: int) -> int:
+    """The address of a per-row vector on GPU ``index``, 0 for none."""
     if t is None:
-        return None
-    if t.device != device or t.dtype != torch.float32 or t.shape != (rows,) \
-            or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous float32 [{rows}] on the logits' GPU")
+        return 0
+    if t.get_device() != index or t.dtype is not dtype or t.shape != (rows,) \
+            or (rows > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what} must be contiguous {dtype} [{rows}] on the logits' GPU")
     return t.data_ptr()
 
 
-def _row_matrix(t: torch.Tensor, what: str, device: torch.device) -> int:
-    """t's row stride, checked to be a matrix of contiguous rows on the logits' GPU."""
-    if t.dim() != 2 or t.device != device or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what} must be a matrix with contiguous rows on the logits' GPU")
-    return N.row_stride(t)
-
-
-def _index(t: torch.Tensor | None, rows: int, what: str, device: torch.device) -> int | None:
-    if t is None:
-        return None
-    if t.device != device or t.dtype != torch.int64 or t.shape != (rows,) or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous int64 [{rows}] on the logits' GPU")
-    return t.data_ptr()
+def _row_stride(t: torch.Tensor, what: str, index: int) -> int:
+    """The row stride of a matrix with contiguous rows on GPU ``index``."""
+    strides = t.stride()
+    if t.get_device() != index or len(strides) != 2:
+        raise ValueError(f"{what} must be a matrix on the logits' GPU")
+    rows, width = t.shape
+    if strides[1] != 1 and width > 1:
+        raise ValueError(f"{what} must have contiguous rows")
+    return strides[0] if rows > 1 else width
 
 
 def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
@@ -60,76 +55,81 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     count, prompt_lengths [slots] how many of those are the prompt (none by default); slot_index
     [rows] names each row's slot, by default its own. repetition, frequency and presence are float32
     [rows]. Each part is optional. ``out`` (f32 or the logits' dtype) may be the logits."""
-    N.require_device(logits, history, lengths, prompt_lengths, slot_index, repetition, frequency,
-                     presence, bias_tokens, bias_values, allowed, allowed_index, out)
-    device = logits.device
-    if logits.dtype not in _FLOATS:
+    index = logits.get_device()
+    if index < 0:
+        N.require_device(logits)
+    dtype = logits.dtype
+    if dtype not in _FLOATS:
         raise ValueError("logits must be f32, bf16 or f16")
-    stride = _row_matrix(logits, "logits", device)
+    stride = _row_stride(logits, "logits", index)
     rows, vocab = logits.shape
     if vocab < 1:
         raise ValueError("logits have no vocabulary")
     if out is None:
-        out = torch.empty(rows, vocab, dtype=logits.dtype, device=device)
-    elif out.shape != logits.shape or out.dtype not in (logits.dtype, torch.float32):
-        raise ValueError("out must be like the logits, or float32")
-    out_stride = _row_matrix(out, "out", device)
-    penalties = [_per_row(t, rows, what, device)
-                 for t, what in ((repetition, "repetition"), (frequency, "frequency"),
-                                 (presence, "presence"))]
+        out = torch.empty((rows, vocab), dtype=dtype, device=logits.device)
+        out_dtype, out_stride = dtype, vocab
+    else:
+        out_dtype = out.dtype
+        if out.shape != logits.shape or (out_dtype is not dtype and out_dtype is not torch.float32):
+            raise ValueError("out must be like the logits, or float32")
+        out_stride = _row_stride(out, "out", index)
     tokens_dtype = lengths_dtype = torch.int32
-    history_stride = capacity = slots = 0
+    history_ptr = history_stride = capacity = slots = lengths_ptr = prompt_ptr = 0
     if history is None:
-        if any(t is not None for t in (lengths, prompt_lengths, slot_index, *penalties)):
+        if not (lengths is None and prompt_lengths is None and slot_index is None
+                and repetition is None and frequency is None and presence is None):
             raise ValueError("lengths, slots and penalties go with a history")
     else:
-        history_stride = _row_matrix(history, "history", device)
+        history_stride = _row_stride(history, "history", index)
         slots, capacity = history.shape
         tokens_dtype = history.dtype
-        if tokens_dtype not in _INTS or lengths is None:
-            raise ValueError("history must be int32 or int64 and come with lengths")
+        if tokens_dtype not in _INTS or lengths is None or lengths.dtype not in _INTS:
+            raise ValueError("history must be int32 or int64 and come with lengths of such a dtype")
         lengths_dtype = lengths.dtype
-        for t, what in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths")):
-            if t is not None and (t.dtype not in _INTS or t.dtype != lengths_dtype
-                                  or t.shape != (slots,) or not t.is_contiguous()
-                                  or t.device != device):
-                raise ValueError(f"{what} must be contiguous int32 or int64 [{slots}], both alike")
+        lengths_ptr = _per_row(lengths, slots, lengths_dtype, "lengths", index)
+        prompt_ptr = _per_row(prompt_lengths, slots, lengths_dtype, "prompt_lengths", index)
         if slot_index is None and slots < rows:
             raise ValueError(f"{slots} histories for {rows} rows need a slot_index")
-    biases = tokens_stride = values_stride = 0
-    if (bias_tokens is None) != (bias_values is None):
-        raise ValueError("bias_tokens and bias_values come together")
-    if bias_tokens is not None:
-        tokens_stride = _row_matrix(bias_tokens, "bias_tokens", device)
-        values_stride = _row_matrix(bias_values, "bias_values", device)
+        history_ptr = history.data_ptr()
+    bias_ptr = values_ptr = biases = tokens_stride = values_stride = 0
+    if bias_tokens is not None and bias_values is not None:
+        tokens_stride = _row_stride(bias_tokens, "bias_tokens", index)
+        values_stride = _row_stride(bias_values, "bias_values", index)
+        bias_dtype = bias_tokens.dtype
         if (bias_tokens.shape != bias_values.shape or bias_tokens.shape[0] != rows
-                or bias_values.dtype != torch.float32 or bias_tokens.dtype not in _INTS
-                or (history is not None and bias_tokens.dtype != tokens_dtype)):
+                or bias_values.dtype is not torch.float32 or bias_dtype not in _INTS
+                or (history is not None and bias_dtype is not tokens_dtype)):
             raise ValueError("bias_tokens (int32 or int64, as the history) and bias_values "
                              "(float32) must be [rows, entries] alike")
-        tokens_dtype = bias_tokens.dtype
+        tokens_dtype = bias_dtype
         biases = bias_tokens.shape[1]
-    masks = allowed_stride = 0
+        bias_ptr, values_ptr = bias_tokens.data_ptr(), bias_values.data_ptr()
+    elif bias_tokens is not None or bias_values is not None:
+        raise ValueError("bias_tokens and bias_values come together")
+    allowed_ptr = masks = allowed_stride = 0
     if allowed is not None:
-        allowed_stride = _row_matrix(allowed, "allowed", device)
-        masks = allowed.shape[0]
-        if allowed.dtype != torch.int32 or allowed.shape[1] < (vocab + 31) // 32:
+        allowed_stride = _row_stride(allowed, "allowed", index)
+        masks, words = allowed.shape
+        if allowed.dtype is not torch.int32 or words < (vocab + 31) // 32:
             raise ValueError(f"allowed must be int32 [masks, {(vocab + 31) // 32}]")
         if allowed_index is None and masks < rows:
             raise ValueError(f"{masks} masks for {rows} rows need an allowed_index")
+        allowed_ptr = allowed.data_ptr()
     elif allowed_index is not None:
         raise ValueError("allowed_index goes with allowed")
-    args = N.LogitsArgs(
-        logits.data_ptr(), N.omni_dtype(logits.dtype), stride, out.data_ptr(),
-        N.omni_dtype(out.dtype), out_stride, rows, vocab, N.ptr(history),
-        N.omni_dtype(tokens_dtype), history_stride, capacity, slots, N.ptr(lengths),
-        N.ptr(prompt_lengths), N.omni_dtype(lengths_dtype),
-        _index(slot_index, rows, "slot_index", device), *penalties, N.ptr(bias_tokens),
-        tokens_stride, N.ptr(bias_values), values_stride, biases, N.ptr(allowed), allowed_stride,
-        masks, _index(allowed_index, rows, "allowed_index", device))
-    lib = N.load_library()
-    N.check(lib.omni_adjust_logits(ctypes.byref(args), N.stream_handle(device)),
-            "omni_adjust_logits")
+    codes, f32, i64 = N.TORCH_TO_OMNI, torch.float32, torch.int64
+    args = N.pack_logits(
+        logits.data_ptr(), codes[dtype], stride, out.data_ptr(), codes[out_dtype], out_stride, rows,
+        vocab, history_ptr, codes[tokens_dtype], history_stride, capacity, slots, lengths_ptr,
+        prompt_ptr, codes[lengths_dtype], _per_row(slot_index, rows, i64, "slot_index", index),
+        _per_row(repetition, rows, f32, "repetition", index),
+        _per_row(frequency, rows, f32, "frequency", index),
+        _per_row(presence, rows, f32, "presence", index), bias_ptr, tokens_stride, values_ptr,
+        values_stride, biases, allowed_ptr, allowed_stride, masks,
+        _per_row(allowed_index, rows, i64, "allowed_index", index))
+    status = N.load_library().omni_adjust_logits(args, N.raw_stream(index))
+    if status:
+        N.check(status, "omni_adjust_logits")
     return out
 
 

@@ -4,7 +4,6 @@ frequencies, so they stay exact at any position a context reaches."""
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Any, Mapping
 
@@ -81,9 +80,12 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0,
     return inv.to(device) if device is not None else inv, cos_factor
 
 
-def _check_heads(t: torch.Tensor, name: str) -> None:
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+def _heads(t: torch.Tensor, name: str) -> tuple[int, int]:
+    """The token and head strides of [tokens, heads, dim] with contiguous dim."""
+    strides = t.stride()
+    if len(strides) != 3 or (strides[2] != 1 and t.shape[2] > 1):
         raise ValueError(f"{name} must be [tokens, heads, dim] with contiguous dim")
+    return strides[0], strides[1]
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
@@ -98,54 +100,60 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     len(inv_freq)) in the "half" layout and (2 i, 2 i + 1) "interleaved". ``transposed`` turns back
     (by the negative angle), which is the gradient. bf16, f16 or f32; views of a qkv buffer are
     taken as they are; q_out / k_out may be q / k themselves."""
-    N.require_device(q, k, positions, inv_freq, q_out, k_out)
-    _check_heads(q, "q")
-    tokens, heads, dim = q.shape
-    device, dtype = q.device, q.dtype
-    if dtype not in _FLOATS:
-        raise ValueError("q must be bf16, f16 or f32")
+    index = q.get_device()
+    if index < 0 or positions.get_device() != index or inv_freq.get_device() != index \
+            or (k is not None and k.get_device() != index):
+        N.require_device(q, k, positions, inv_freq)
+        raise ValueError("q, k, positions and inv_freq must be on one GPU")
+    q_token, q_head = _heads(q, "q")
+    shape, dtype = q.shape, q.dtype
+    tokens, heads, dim = shape
+    if dtype not in _FLOATS or heads < 1:
+        raise ValueError("q must be bf16, f16 or f32, with at least one head")
     if layout not in _LAYOUTS:
         raise ValueError(f"unknown layout {layout!r}")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be contiguous float64 [pairs]")
     pairs = inv_freq.shape[0]
     if pairs < 1 or 2 * pairs > dim:
         raise ValueError(f"{pairs} pairs do not fit heads of {dim}")
-    if positions.shape != (tokens,) or positions.dtype not in (torch.int32, torch.int64):
+    positions_dtype = positions.dtype
+    if positions.shape != (tokens,) or (positions_dtype is not torch.int64
+                                        and positions_dtype is not torch.int32):
         raise ValueError(f"positions must be int32 or int64 [{tokens}]")
-    if positions.device != device or inv_freq.device != device:
-        raise ValueError("q, positions and inv_freq must be on one GPU")
-    if heads < 1:
-        raise ValueError("q has no heads")
     if q_out is None:
-        q_out = torch.empty(tokens, heads, dim, dtype=dtype, device=device)
+        q_out = torch.empty(shape, dtype=dtype, device=q.device)
+        qo_token, qo_head = heads * dim, dim
     else:
-        _check_heads(q_out, "q_out")
-        if q_out.shape != q.shape or q_out.dtype != dtype or q_out.device != device:
+        qo_token, qo_head = _heads(q_out, "q_out")
+        if q_out.shape != shape or q_out.dtype is not dtype or q_out.get_device() != index:
             raise ValueError("q_out must be like q")
-    kv_heads, k_ptr, k_t, k_h, ko_ptr, ko_t, ko_h = 0, None, 0, 0, None, 0, 0
+    kv_heads = k_ptr = k_token = k_head = ko_ptr = ko_token = ko_head = 0
     if k is not None:
-        _check_heads(k, "k")
-        kv_heads = k.shape[1]
-        if k.shape[0] != tokens or k.shape[2] != dim or k.dtype != dtype or k.device != device:
-            raise ValueError("k must be [tokens, kv_heads, dim] of q's dtype and device")
+        k_token, k_head = _heads(k, "k")
+        k_shape = k.shape
+        kv_heads = k_shape[1]
+        if k_shape[0] != tokens or k_shape[2] != dim or k.dtype is not dtype:
+            raise ValueError("k must be [tokens, kv_heads, dim] of q's dtype")
         if k_out is None:
-            k_out = torch.empty(tokens, kv_heads, dim, dtype=dtype, device=device)
+            k_out = torch.empty(k_shape, dtype=dtype, device=q.device)
+            ko_token, ko_head = kv_heads * dim, dim
         else:
-            _check_heads(k_out, "k_out")
-            if k_out.shape != k.shape or k_out.dtype != dtype or k_out.device != device:
+            ko_token, ko_head = _heads(k_out, "k_out")
+            if k_out.shape != k_shape or k_out.dtype is not dtype or k_out.get_device() != index:
                 raise ValueError("k_out must be like k")
-        k_ptr, k_t, k_h = k.data_ptr(), k.stride(0), k.stride(1)
-        ko_ptr, ko_t, ko_h = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
+        k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         raise ValueError("k_out goes with k")
-    args = N.RotaryArgs(q.data_ptr(), q.stride(0), q.stride(1), k_ptr, k_t, k_h, q_out.data_ptr(),
-                        q_out.stride(0), q_out.stride(1), ko_ptr, ko_t, ko_h, N.omni_dtype(dtype),
-                        tokens, heads, kv_heads, dim, pairs, positions.data_ptr(),
-                        N.omni_dtype(positions.dtype), positions.stride(0), inv_freq.data_ptr(),
-                        factor, _LAYOUTS[layout], int(transposed))
-    lib = N.load_library()
-    N.check(lib.omni_rotary(ctypes.byref(args), N.stream_handle(device)), "omni_rotary")
+    codes = N.TORCH_TO_OMNI
+    args = N.pack_rotary(
+        q.data_ptr(), q_token, q_head, k_ptr, k_token, k_head, q_out.data_ptr(), qo_token, qo_head,
+        ko_ptr, ko_token, ko_head, codes[dtype], tokens, heads, kv_heads, dim, pairs,
+        positions.data_ptr(), codes[positions_dtype], positions.stride(0), inv_freq.data_ptr(),
+        factor, _LAYOUTS[layout], 1 if transposed else 0)
+    status = N.load_library().omni_rotary(args, N.raw_stream(index))
+    if status:
+        N.check(status, "omni_rotary")
     return q_out if k is None else (q_out, k_out)
 
 
