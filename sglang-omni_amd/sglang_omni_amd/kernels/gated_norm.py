@@ -18,8 +18,8 @@ def _vector(t: torch.Tensor | None, channels: int, index: int, what: str) -> int
     """The address of a per-channel float32 vector on GPU ``index``, 0 for none."""
     if t is None:
         return 0
-    if t.dtype is not torch.float32 or t.shape != (channels,) or t.get_device() != index \
-            or (channels > 1 and t.stride(0) != 1):
+    if t.dtype is not torch.float32 or t.numel() != channels or t.get_device() != index \
+            or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous float32 [{channels}] on x's GPU")
     return t.data_ptr()
 
@@ -49,9 +49,10 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", 
         N.require_device(x, y, gate)
         raise ValueError("x, y and gate must be on one GPU")
     x_dtype, y_dtype = x.dtype, y.dtype
-    if x.dim() != 2 or x.shape != y.shape:
+    shape = x.shape
+    if len(shape) != 2 or shape != y.shape:
         raise ValueError("x and y must be [rows, channels] alike")
-    rows, c = x.shape
+    rows, c = shape
     x_stride, x_contiguous = x.stride()
     y_stride, y_contiguous = y.stride()
     if c < 1 or (c > 1 and (x_contiguous != 1 or y_contiguous != 1)):
@@ -66,37 +67,40 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", 
         raise ValueError("post_weight and post_bias go with post_norm")
     gate_ptr, gate_code, gate_stride, rows_per_gate = 0, N.DTYPE_F32, 0, 1
     if gate is not None:
-        gate_shape = gate.shape
+        gate_shape, gate_strides = gate.shape, gate.stride()
         gates = gate_shape[0] if len(gate_shape) == 2 else 1
         if (len(gate_shape) not in (1, 2) or gate_shape[-1] != c or gate.dtype not in _FLOATS
-                or (c > 1 and gate.stride(-1) != 1) or gates < 1 or rows % gates):
+                or (c > 1 and gate_strides[-1] != 1) or gates < 1 or rows % gates):
             raise ValueError("gate must be bf16, f16 or f32 [channels] or [G, channels], rows a "
                              "multiple of G, with contiguous rows")
         gate_ptr, gate_code = gate.data_ptr(), N.TORCH_TO_OMNI[gate.dtype]
         if gates > 1:
-            gate_stride = gate.stride(0)  # 0 for a gate expanded over its rows
+            gate_stride = gate_strides[0]  # 0 for a gate expanded over its rows
         rows_per_gate = max(rows // gates, 1)
     elif gate_activation != "none":
         raise ValueError("gate_activation goes with a gate")
-    device = x.device
     if residual_out is None:
-        residual_out = torch.empty((rows, c), dtype=x_dtype, device=device)
-        out_stride = c
+        residual_out = torch.empty_like(x)
+        out_stride = residual_out.stride(0) if rows > 1 else c
     else:
-        if (residual_out.shape != x.shape or residual_out.dtype is not x_dtype
+        if (residual_out.shape != shape or residual_out.dtype is not x_dtype
                 or (c > 1 and residual_out.stride(1) != 1) or residual_out.get_device() != index):
             raise ValueError("residual_out must be like x, with contiguous rows")
         out_stride = N.row_stride(residual_out)
     if normed_dtype is None:
         normed_dtype = y_dtype
-    normed_scale, scale_ptr, scale_stride, normed_width = None, 0, 0, c
-    if normed_dtype is torch.float8_e4m3fn:
-        normed_width, scale_stride = (c + 15) // 16 * 16, (c + BLOCK - 1) // BLOCK
-        normed_scale = torch.empty((rows, scale_stride), dtype=torch.float32, device=device)
+    normed_scale, scale_ptr, scale_stride = None, 0, 0
+    if normed_dtype is y_dtype:
+        normed = torch.empty_like(y)
+    elif normed_dtype in _FLOATS:
+        normed = torch.empty(shape, dtype=normed_dtype, device=x.device)
+    elif normed_dtype is torch.float8_e4m3fn:
+        normed = torch.empty((rows, (c + 15) // 16 * 16), dtype=normed_dtype, device=x.device)
+        scale_stride = (c + BLOCK - 1) // BLOCK
+        normed_scale = torch.empty((rows, scale_stride), dtype=torch.float32, device=x.device)
         scale_ptr = normed_scale.data_ptr()
-    elif normed_dtype not in _FLOATS:
+    else:
         raise ValueError("normed_dtype must be bf16, f16, f32 or float8_e4m3fn")
-    normed = torch.empty((rows, normed_width), dtype=normed_dtype, device=device)
     codes = N.TORCH_TO_OMNI
     args = N.pack_gated_norm(
         x.data_ptr(), codes[x_dtype], x_stride if rows > 1 else c, y.data_ptr(), codes[y_dtype],
@@ -104,8 +108,8 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", 
         _vector(post_weight, c, index, "post_weight"), _vector(post_bias, c, index, "post_bias"),
         _vector(pre_weight, c, index, "pre_weight"), _vector(pre_bias, c, index, "pre_bias"),
         gate_ptr, gate_code, gate_stride, rows_per_gate, _ACTIVATIONS[gate_activation],
-        residual_out.data_ptr(), out_stride, normed.data_ptr(), codes[normed_dtype], normed_width,
-        scale_ptr, scale_stride)
+        residual_out.data_ptr(), out_stride, normed.data_ptr(), codes[normed_dtype],
+        N.row_stride(normed), scale_ptr, scale_stride)
     status = N.load_library().omni_gated_residual_norm(args, N.raw_stream(index))
     if status:
         N.check(status, "omni_gated_residual_norm")

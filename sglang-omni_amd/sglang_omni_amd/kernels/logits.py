@@ -15,8 +15,8 @@ def _per_row(t: torch.Tensor | None, rows: int, dtype: torch.dtype, what: str, i
     """The address of a per-row vector on GPU ``index``, 0 for none."""
     if t is None:
         return 0
-    if t.get_device() != index or t.dtype is not dtype or t.shape != (rows,) \
-            or (rows > 1 and t.stride(0) != 1):
+    if t.get_device() != index or t.dtype is not dtype or t.numel() != rows \
+            or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {dtype} [{rows}] on the logits' GPU")
     return t.data_ptr()
 
@@ -66,8 +66,8 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     if vocab < 1:
         raise ValueError("logits have no vocabulary")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=dtype, device=logits.device)
-        out_dtype, out_stride = dtype, vocab
+        out = torch.empty_like(logits)
+        out_dtype, out_stride = dtype, N.row_stride(out)
     else:
         out_dtype = out.dtype
         if out.shape != logits.shape or (out_dtype is not dtype and out_dtype is not torch.float32):

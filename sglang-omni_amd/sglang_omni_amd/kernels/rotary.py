@@ -118,12 +118,12 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if pairs < 1 or 2 * pairs > dim:
         raise ValueError(f"{pairs} pairs do not fit heads of {dim}")
     positions_dtype = positions.dtype
-    if positions.shape != (tokens,) or (positions_dtype is not torch.int64
+    if positions.dim() != 1 or positions.shape[0] != tokens or (positions_dtype is not torch.int64
                                         and positions_dtype is not torch.int32):
         raise ValueError(f"positions must be int32 or int64 [{tokens}]")
     if q_out is None:
-        q_out = torch.empty(shape, dtype=dtype, device=q.device)
-        qo_token, qo_head = heads * dim, dim
+        q_out = torch.empty_like(q)  # dense, in q's order of tokens and heads
+        qo_token, qo_head, _ = q_out.stride()
     else:
         qo_token, qo_head = _heads(q_out, "q_out")
         if q_out.shape != shape or q_out.dtype is not dtype or q_out.get_device() != index:
@@ -136,8 +136,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if k_shape[0] != tokens or k_shape[2] != dim or k.dtype is not dtype:
             raise ValueError("k must be [tokens, kv_heads, dim] of q's dtype")
         if k_out is None:
-            k_out = torch.empty(k_shape, dtype=dtype, device=q.device)
-            ko_token, ko_head = kv_heads * dim, dim
+            k_out = torch.empty_like(k)
+            ko_token, ko_head, _ = k_out.stride()
         else:
             ko_token, ko_head = _heads(k_out, "k_out")
             if k_out.shape != k_shape or k_out.dtype is not dtype or k_out.get_device() != index:

@@ -91,6 +91,16 @@ def test_linear(gpu, rows, k, n, out):
     _check(block_fp8_linear(q, w, out_dtype=out), q, w)
 
 
+@pytest.mark.parametrize("rows,k,n", [(300, 272, 4100), (530, 400, 4097), (2100, 272, 4100), (4099, 144, 3075),
+                                      (700, 2064, 1300)])
+def test_larger_tiles(gpu, rows, k, n):
+    """Sizes that the tiles of 64 x 128, 128 x 128 and 256 x 256 take, ragged in every direction."""
+    x, w = _operands(gpu, rows, k, n, rows, bias=True)
+    q = quantize_block_rows(x)
+    for out in (torch.bfloat16, torch.float32):
+        _check(block_fp8_linear(q, w, out_dtype=out), q, w)
+
+
 @pytest.mark.parametrize("rows", [1, 16, 64, 200])
 def test_operands_over_all_binades(gpu, rows):
     """Any E4M3 bit patterns. float32 output keeps the float32 bound. bf16 output may lose what the

@@ -178,6 +178,19 @@ def test_long_history_counts(gpu):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("entries", [1, 63, 65, 130, 600, 1100])
+@pytest.mark.parametrize("vocab", [40, 9001, 20000])
+def test_long_bias_lists_with_repeats(gpu, entries, vocab):
+    """Lists shorter and longer than a wave and than a workgroup; most tokens named several times."""
+    g = torch.Generator().manual_seed(entries + vocab)
+    logits, kw = _inputs(gpu, 2, vocab, 300, entries)
+    tokens = torch.randint(-1, min(vocab, 200), (2, entries), generator=g)
+    tokens[1] *= max(1, vocab // 200)
+    kw["bias_tokens"] = tokens.to(torch.int32).to(gpu)
+    kw["bias_values"] = (torch.randn(2, entries, generator=g) * 5).to(gpu)
+    _check(logits, **kw)
+
+
 def test_strides_outputs_and_in_place(gpu):
     logits, kw = _inputs(gpu, 5, 3001, 64, 13)
     want = adjust_logits(logits, **kw)
