@@ -70,10 +70,14 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   const int64_t token = rest / p.groups;
   const int head0 = (int)(rest - token * p.groups) * kHeadsPerThread;
   const bool turned = chunk < p.turned_chunks;
-  // the chunk's two runs of V values
-  const int past = 2 * p.pairs + (chunk - p.turned_chunks) * 2 * V;
-  const int at0 = turned ? (INTERLEAVED ? chunk * 2 * V : chunk * V) : past;
-  const int at1 = turned && !INTERLEAVED ? at0 + p.pairs : at0 + V;
+  // the chunk's two runs of V values, neighbours' runs side by side: in the half layout the pairs'
+  // first and second values; interleaved (V > 1), V / 2 pairs of the first half of the pairs and as
+  // many of the second; of what is copied, one run of each half (in turn where it has no halves)
+  const int past = 2 * p.pairs, rest_dim = p.dim - past, copied = chunk - p.turned_chunks;
+  const bool halves = rest_dim % (2 * V) == 0;
+  const int at0 = turned ? chunk * (INTERLEAVED && V == 1 ? 2 : V) : past + copied * (halves ? V : 2 * V);
+  const int at1 = turned ? (INTERLEAVED && V == 1 ? at0 + 1 : at0 + p.pairs)
+                         : at0 + (halves ? rest_dim / 2 : V);
   const int64_t valid1 = p.dim - at1;  // a copied run may end with the head
 
   const T* src[kHeadsPerThread];
@@ -99,7 +103,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
     float s[V], c[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      sincos_turn(position * p.inv_freq[chunk * V + v] * 0.15915494309189535, &s[v], &c[v]);
+      const int i = !INTERLEAVED || V == 1 ? chunk * V + v
+                    : v < V / 2            ? chunk * (V / 2) + v
+                                           : p.pairs / 2 + chunk * (V / 2) + v - V / 2;
+      sincos_turn(position * p.inv_freq[i] * 0.15915494309189535, &s[v], &c[v]);
       s[v] *= p.negative ? -p.factor : p.factor;
       c[v] *= p.factor;
     }

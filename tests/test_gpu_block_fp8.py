@@ -94,11 +94,16 @@ def test_linear(gpu, rows, k, n, out):
 @pytest.mark.parametrize("rows,k,n", [(300, 272, 4100), (530, 400, 4097), (2100, 272, 4100), (4099, 144, 3075),
                                       (700, 2064, 1300)])
 def test_larger_tiles(gpu, rows, k, n):
-    """Sizes that the tiles of 64 x 128, 128 x 128 and 256 x 256 take, ragged in every direction."""
+    """Sizes that the tiles of 64 x 128, 128 x 128 and 256 x 256 take, ragged in every direction:
+    float32 against float64, and bf16, whose products the 8-bit instruction cuts, against the bits of
+    the small tiles on 40 rows at a time (every tile adds an element's blocks in one order)."""
     x, w = _operands(gpu, rows, k, n, rows, bias=True)
     q = quantize_block_rows(x)
-    for out in (torch.bfloat16, torch.float32):
-        _check(block_fp8_linear(q, w, out_dtype=out), q, w)
+    _check(block_fp8_linear(q, w, out_dtype=torch.float32), q, w)
+    whole = block_fp8_linear(q, w)
+    for at in (0, rows // 2, rows - 40):
+        part = BlockFp8Rows(q.values[at:at + 40], q.scale[at:at + 40])
+        assert torch.equal(block_fp8_linear(part, w), whole[at:at + 40])
 
 
 @pytest.mark.parametrize("rows", [1, 16, 64, 200])
