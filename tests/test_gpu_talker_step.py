@@ -8,7 +8,8 @@ from pathlib import Path
 import pytest
 import torch
 
-from sglang_omni_amd.kernels import block_fp8_linear
+from sglang_omni_amd.kernels import (adjust_logits, apply_rotary, block_fp8_linear,
+                                     gated_residual_norm, pack_block_fp8, rotary_frequencies)
 from sglang_omni_amd.models import DacCodecDecoder, DacDecoderConfig, make_dac_weights
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +89,45 @@ def test_penalties_change_the_choice(gpu, example):
     held = example.Talker(config, 1, gpu).codes(1, 40, repetition=1e6)[0, 0]
     assert free.unique().numel() < 40
     assert held.unique().numel() == 40
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_captured_in_a_graph_and_on_a_side_stream(gpu, rows):
+    """One capture of the four operators in a row, replayed on new inputs between eager work, and the
+    same on a stream that is not the default one."""
+    g = torch.Generator().manual_seed(rows)
+    w = pack_block_fp8(torch.randn(512, 256, generator=g)).to(gpu)
+    inv, _ = rotary_frequencies(64, device=gpu)
+    x = torch.randn(rows, 256, generator=g).to(gpu)
+    y = torch.randn(rows, 256, generator=g).to(torch.bfloat16).to(gpu)
+    positions = torch.arange(rows, device=gpu)
+    history = torch.randint(0, 512, (rows, 30), generator=g).to(gpu)
+    lengths = torch.full((rows,), 30, device=gpu)
+    penalty = torch.full((rows,), 1.5, device=gpu)
+
+    def step():
+        h, n = gated_residual_norm(x, y, post_norm=True, normed_dtype=torch.float8_e4m3fn)
+        q = block_fp8_linear(n, w)
+        r = apply_rotary(q.view(rows, 8, 64), None, positions, inv)
+        z = block_fp8_linear(y, w, out_dtype=torch.float32)
+        return h, q, r, adjust_logits(z, history=history, lengths=lengths, repetition=penalty)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            aside = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(aside, step()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        x.copy_(torch.randn(rows, 256, generator=g))
+        y.copy_(torch.randn(rows, 256, generator=g))
+        positions += k
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
