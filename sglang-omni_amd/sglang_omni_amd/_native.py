@@ -503,11 +503,12 @@ def require_slot_state(history: torch.Tensor | None, slot_index: torch.Tensor | 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def raw_stream(index: int) -> int:
-    """The current stream's handle on GPU ``index``."""
-    if _raw_stream is not None:
-        return _raw_stream(index)
+def _stream_of(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
+
+
+# The current stream's handle on GPU `index`.
+raw_stream = _raw_stream if _raw_stream is not None else _stream_of
 
 
 def stream_handle(device: torch.device | None = None) -> int:

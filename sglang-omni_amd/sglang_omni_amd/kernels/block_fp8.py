@@ -15,6 +15,8 @@ from .. import _native as N
 BLOCK = 128
 _E4M3 = torch.float8_e4m3fn
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_CODES, _pack, _raw_stream = N.TORCH_TO_OMNI, N.pack_block_fp8, N.raw_stream
+_launch = None  # the entry point, bound at the first call
 
 
 @dataclass
@@ -161,14 +163,16 @@ def block_fp8_linear(x: torch.Tensor | BlockFp8Rows, weight: BlockFp8Weight,
         if out.shape != (rows, n) or (n > 1 and out.stride(1) != 1) or out_dtype not in _FLOATS:
             raise ValueError(f"out must be bf16, f16 or f32 [{rows}, {n}] with contiguous rows")
         out_stride = N.row_stride(out)
-    codes = N.TORCH_TO_OMNI
-    args = N.pack_block_fp8(
-        values.data_ptr(), codes[values.dtype], x_stride if rows > 1 else features, features,
+    args = _pack(
+        values.data_ptr(), _CODES[values.dtype], x_stride if rows > 1 else features, features,
         scale_ptr, scale_row, scale_block, w.data_ptr(), w_stride if n > 1 else k,
         w_scale.data_ptr(), N.row_stride(w_scale), rows, n, k,
-        0 if bias is None else bias.data_ptr(), out.data_ptr(), out_stride, codes[out_dtype],
+        0 if bias is None else bias.data_ptr(), out.data_ptr(), out_stride, _CODES[out_dtype],
         0 if workspace is None else workspace.data_ptr(), workspace_bytes)
-    status = N.load_library().omni_block_fp8_gemm(args, N.raw_stream(index))
+    global _launch
+    if _launch is None:
+        _launch = N.load_library().omni_block_fp8_gemm
+    status = _launch(args, _raw_stream(index))
     if status:
         N.check(status, "omni_block_fp8_gemm")
     return out

@@ -10,6 +10,8 @@ from .. import _native as N
 from .block_fp8 import BLOCK, BlockFp8Rows
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_CODES, _pack, _raw_stream = N.TORCH_TO_OMNI, N.pack_gated_norm, N.raw_stream
+_launch = None  # the entry point, bound at the first call
 _NORMS = {"rms": N.NORM_RMS, "layer": N.NORM_LAYER}
 _ACTIVATIONS = {"none": N.GATE_NONE, "sigmoid": N.GATE_SIGMOID, "tanh": N.GATE_TANH}
 
@@ -73,7 +75,7 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", 
                 or (c > 1 and gate_strides[-1] != 1) or gates < 1 or rows % gates):
             raise ValueError("gate must be bf16, f16 or f32 [channels] or [G, channels], rows a "
                              "multiple of G, with contiguous rows")
-        gate_ptr, gate_code = gate.data_ptr(), N.TORCH_TO_OMNI[gate.dtype]
+        gate_ptr, gate_code = gate.data_ptr(), _CODES[gate.dtype]
         if gates > 1:
             gate_stride = gate_strides[0]  # 0 for a gate expanded over its rows
         rows_per_gate = max(rows // gates, 1)
@@ -101,16 +103,18 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, *, norm: str = "rms", 
         scale_ptr = normed_scale.data_ptr()
     else:
         raise ValueError("normed_dtype must be bf16, f16, f32 or float8_e4m3fn")
-    codes = N.TORCH_TO_OMNI
-    args = N.pack_gated_norm(
-        x.data_ptr(), codes[x_dtype], x_stride if rows > 1 else c, y.data_ptr(), codes[y_dtype],
+    args = _pack(
+        x.data_ptr(), _CODES[x_dtype], x_stride if rows > 1 else c, y.data_ptr(), _CODES[y_dtype],
         y_stride if rows > 1 else c, rows, c, _NORMS[norm], 1 if post_norm else 0, eps, scale,
         _vector(post_weight, c, index, "post_weight"), _vector(post_bias, c, index, "post_bias"),
         _vector(pre_weight, c, index, "pre_weight"), _vector(pre_bias, c, index, "pre_bias"),
         gate_ptr, gate_code, gate_stride, rows_per_gate, _ACTIVATIONS[gate_activation],
-        residual_out.data_ptr(), out_stride, normed.data_ptr(), codes[normed_dtype],
+        residual_out.data_ptr(), out_stride, normed.data_ptr(), _CODES[normed_dtype],
         N.row_stride(normed), scale_ptr, scale_stride)
-    status = N.load_library().omni_gated_residual_norm(args, N.raw_stream(index))
+    global _launch
+    if _launch is None:
+        _launch = N.load_library().omni_gated_residual_norm
+    status = _launch(args, _raw_stream(index))
     if status:
         N.check(status, "omni_gated_residual_norm")
     return residual_out, normed if normed_scale is None else BlockFp8Rows(normed, normed_scale)

@@ -8,6 +8,8 @@ import torch
 from .. import _native as N
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_CODES, _pack, _raw_stream = N.TORCH_TO_OMNI, N.pack_logits, N.raw_stream
+_launch = None  # the entry point, bound at the first call
 _INTS = (torch.int32, torch.int64)
 
 
@@ -117,17 +119,20 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         allowed_ptr = allowed.data_ptr()
     elif allowed_index is not None:
         raise ValueError("allowed_index goes with allowed")
-    codes, f32, i64 = N.TORCH_TO_OMNI, torch.float32, torch.int64
-    args = N.pack_logits(
-        logits.data_ptr(), codes[dtype], stride, out.data_ptr(), codes[out_dtype], out_stride, rows,
-        vocab, history_ptr, codes[tokens_dtype], history_stride, capacity, slots, lengths_ptr,
-        prompt_ptr, codes[lengths_dtype], _per_row(slot_index, rows, i64, "slot_index", index),
+    f32, i64 = torch.float32, torch.int64
+    args = _pack(
+        logits.data_ptr(), _CODES[dtype], stride, out.data_ptr(), _CODES[out_dtype], out_stride, rows,
+        vocab, history_ptr, _CODES[tokens_dtype], history_stride, capacity, slots, lengths_ptr,
+        prompt_ptr, _CODES[lengths_dtype], _per_row(slot_index, rows, i64, "slot_index", index),
         _per_row(repetition, rows, f32, "repetition", index),
         _per_row(frequency, rows, f32, "frequency", index),
         _per_row(presence, rows, f32, "presence", index), bias_ptr, tokens_stride, values_ptr,
         values_stride, biases, allowed_ptr, allowed_stride, masks,
         _per_row(allowed_index, rows, i64, "allowed_index", index))
-    status = N.load_library().omni_adjust_logits(args, N.raw_stream(index))
+    global _launch
+    if _launch is None:
+        _launch = N.load_library().omni_adjust_logits
+    status = _launch(args, _raw_stream(index))
     if status:
         N.check(status, "omni_adjust_logits")
     return out

@@ -12,6 +12,8 @@ import torch
 from .. import _native as N
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_CODES, _pack, _raw_stream = N.TORCH_TO_OMNI, N.pack_rotary, N.raw_stream
+_launch = None  # the entry point, bound at the first call
 _LAYOUTS = {"half": N.ROTARY_HALF, "interleaved": N.ROTARY_INTERLEAVED}
 
 
@@ -145,13 +147,15 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         raise ValueError("k_out goes with k")
-    codes = N.TORCH_TO_OMNI
-    args = N.pack_rotary(
+    args = _pack(
         q.data_ptr(), q_token, q_head, k_ptr, k_token, k_head, q_out.data_ptr(), qo_token, qo_head,
-        ko_ptr, ko_token, ko_head, codes[dtype], tokens, heads, kv_heads, dim, pairs,
-        positions.data_ptr(), codes[positions_dtype], positions.stride(0), inv_freq.data_ptr(),
+        ko_ptr, ko_token, ko_head, _CODES[dtype], tokens, heads, kv_heads, dim, pairs,
+        positions.data_ptr(), _CODES[positions_dtype], positions.stride(0), inv_freq.data_ptr(),
         factor, _LAYOUTS[layout], 1 if transposed else 0)
-    status = N.load_library().omni_rotary(args, N.raw_stream(index))
+    global _launch
+    if _launch is None:
+        _launch = N.load_library().omni_rotary
+    status = _launch(args, _raw_stream(index))
     if status:
         N.check(status, "omni_rotary")
     return q_out if k is None else (q_out, k_out)
