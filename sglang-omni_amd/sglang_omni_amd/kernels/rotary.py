@@ -17,6 +17,23 @@ _launch = None  # the entry point, bound at the first call
 _LAYOUTS = {"half": N.ROTARY_HALF, "interleaved": N.ROTARY_INTERLEAVED}
 
 
+# The keys of each kind of scaling. Another key would change what the configuration means, so it is
+# refused rather than passed over.
+_SCALING_KEYS = {
+    "default": set(),
+    "linear": {"factor"},
+    "llama3": {"factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"},
+    "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
+             "attention_factor", "mscale", "mscale_all_dim", "truncate"},
+    "longrope": {"factor", "original_max_position_embeddings", "attention_factor", "long_factor",
+                 "short_factor", "short"},
+}
+
+
+def _yarn_magnitude(factor: float, mscale: float) -> float:
+    return 0.1 * mscale * math.log(factor) + 1.0
+
+
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0,
                        scaling: Mapping[str, Any] | None = None,
                        device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
@@ -30,55 +47,95 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0,
       "high_freq_factor" times kept, between them a blend by the turns
     - "yarn": pairs that turn less than "beta_slow" (1) times in the original context divided by
       "factor", those that turn more than "beta_fast" (32) times kept, between them a ramp over the
-      pair index; the factor is "attention_factor" or 0.1 ln(factor) + 1
+      pair index, its ends rounded outwards to whole pairs unless "truncate" is False; the factor is
+      "attention_factor", or m("mscale") / m("mscale_all_dim") where both are given, m(s) = 0.1 s
+      ln(factor) + 1, or else m(1)
     - "longrope": divided by "long_factor" (or "short_factor" with "short": True), one per pair; the
-      factor is "attention_factor" or sqrt(1 + ln(factor) / ln(original context))
-    """
+      factor is "attention_factor" or sqrt(1 + ln(factor) / ln(original context)), where "factor" is
+      the ratio of the model's context to the original one
+
+    A null value is an absent one. "rope_theta" must be ``base``; any other key, a missing "factor"
+    or a missing context (but longrope's with an "attention_factor") is a ValueError: sections of
+    several position rows and a partial head, for instance, are the caller's to apply."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
     if not base > 1.0:
         raise ValueError(f"base must be above 1, got {base}")
     pairs = rotary_dim // 2
     inv = float(base) ** (-torch.arange(pairs, dtype=torch.float64) * 2 / rotary_dim)
-    scaling = dict(scaling or {})
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
-    factor = float(scaling.get("factor", 1.0))
-    if not factor >= 1.0:
-        raise ValueError(f"the scaling factor must be at least 1, got {factor}")
+    scaling = {key: value for key, value in (scaling or {}).items() if value is not None}
+    kinds = {scaling.pop(key) for key in ("rope_type", "type") if key in scaling} or {"default"}
+    kind = kinds.pop()
+    if kinds or kind not in _SCALING_KEYS:
+        raise ValueError(f"unknown rope scaling {' / '.join(map(repr, (kind, *kinds)))}")
+    if float(scaling.pop("rope_theta", base)) != float(base):
+        raise ValueError(f"the rope scaling's rope_theta is not the base {base}")
+    unknown = sorted(scaling.keys() - _SCALING_KEYS[kind])
+    if unknown:
+        raise ValueError(f"{kind} rope scaling does not take {', '.join(unknown)}")
+
+    def number(key: str) -> float:
+        if key not in scaling:
+            raise ValueError(f"{kind} rope scaling needs {key}")
+        return float(scaling[key])
+
+    def context() -> float:
+        original = number("original_max_position_embeddings")
+        if not original > 1.0:
+            raise ValueError(f"the original context must be above 1, got {original}")
+        return original
+
+    factor = 1.0
+    if kind != "default" and not (kind == "longrope" and "attention_factor" in scaling):
+        factor = number("factor")
+        if not factor >= 1.0:
+            raise ValueError(f"the scaling factor must be at least 1, got {factor}")
     cos_factor = 1.0
     if kind == "linear":
         inv = inv / factor
     elif kind == "llama3":
-        original = float(scaling["original_max_position_embeddings"])
-        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        original = context()
+        low, high = number("low_freq_factor"), number("high_freq_factor")
         if not high > low:
             raise ValueError("high_freq_factor must be above low_freq_factor")
         turns = original * inv / (2 * math.pi)
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         inv = inv * (keep + (1 - keep) / factor)
     elif kind == "yarn":
-        original = float(scaling["original_max_position_embeddings"])
+        original = context()
 
         def pair(turns: float) -> float:
             return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low = max(math.floor(pair(float(scaling.get("beta_fast", 32)))), 0)
-        high = min(math.ceil(pair(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
+        low, high = pair(float(scaling.get("beta_fast", 32))), pair(float(scaling.get("beta_slow", 1)))
+        if scaling.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
+        if low > high:  # beta_fast below beta_slow, or a context of less than a turn
+            raise ValueError("yarn's ramp ends before it begins")
         ramp = (torch.arange(pairs, dtype=torch.float64) - low) / max(high - low, 1e-3)
         ramp = ramp.clamp(0, 1)
         inv = inv * (1 - ramp) + inv / factor * ramp
-        cos_factor = float(scaling.get("attention_factor") or 0.1 * math.log(factor) + 1.0)
+        mscale = float(scaling.get("mscale", 1.0))
+        mscale_all_dim = float(scaling.get("mscale_all_dim", 0.0))
+        if "attention_factor" in scaling:
+            cos_factor = float(scaling["attention_factor"])
+        elif mscale and mscale_all_dim and "mscale" in scaling:
+            cos_factor = _yarn_magnitude(factor, mscale) / _yarn_magnitude(factor, mscale_all_dim)
+        elif mscale == 1.0 and mscale_all_dim == 0.0:
+            cos_factor = _yarn_magnitude(factor, 1.0)
+        else:  # the published definitions differ on one without the other
+            raise ValueError("yarn's mscale and mscale_all_dim come together")
     elif kind == "longrope":
         name = "short_factor" if scaling.get("short") else "long_factor"
+        if name not in scaling:
+            raise ValueError(f"longrope rope scaling needs {name}")
         per_pair = torch.as_tensor(scaling[name], dtype=torch.float64)
         if per_pair.shape != (pairs,):
             raise ValueError(f"{name} must hold {pairs} values")
         inv = inv / per_pair
-        original = float(scaling["original_max_position_embeddings"])
-        cos_factor = float(scaling.get("attention_factor")
-                           or math.sqrt(1 + math.log(factor) / math.log(original)))
-    elif kind != "default":
-        raise ValueError(f"unknown rope scaling {kind!r}")
+        cos_factor = (float(scaling["attention_factor"]) if "attention_factor" in scaling
+                      else math.sqrt(1 + math.log(factor) / math.log(context())))
     return inv.to(device) if device is not None else inv, cos_factor
 
 
