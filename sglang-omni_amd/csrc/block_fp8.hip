@@ -531,9 +531,8 @@ int launch_ring(GemmParams p, hipStream_t stream) {
 
 // ------------------------------------------------------------------------------ few rows
 //
-// Up to 16 rows: the weight's bytes are the time, each read once. A workgroup takes 16 columns and
-// TM tiles of 16 rows; its waves take K blocks in turn and load their operands straight into MFMA
-// registers, UNROLL blocks of them in flight, no LDS and no barrier until the waves' sums meet. x is
+// Up to 16 rows: the weight's bytes are the time, each read once. A workgroup takes 16 columns of all
+// rows; its waves take K blocks in turn and load their operands straight into MFMA registers, UNROLL blocks of them in flight, no LDS and no barrier until the waves' sums meet. x is
 // E4M3 rows, or (XT) float rows, whose groups each wave quantizes for itself: the bits of
 // omni_block_quantize without its launch.
 
@@ -585,10 +584,10 @@ OMNI_DEVICE i32x8 quantize_piece(const RowPiece<XT>& piece, float* scale) {
   return bytes;
 }
 
-template <int NW, int TM, int UNROLL, bool EXACT, typename XT>
+template <int NW, int UNROLL, bool EXACT, typename XT>
 __global__ void __launch_bounds__(64 * NW) block_fp8_few_rows_kernel(const GemmParams p) {
   constexpr bool FLOATS = !std::is_same<XT, uint8_t>::value;
-  __shared__ f32x4 sums[NW][TM][64];
+  __shared__ f32x4 sums[NW][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
@@ -598,17 +597,9 @@ __global__ void __launch_bounds__(64 * NW) block_fp8_few_rows_kernel(const GemmP
   const uint32_t w_off = lr < n_rows ? (uint32_t)(lr * (int)p.w_stride + lq * 16) : kOutOfRange;
   const auto xr = buffer_rsrc(p.x, FLOATS ? 0u : (uint32_t)((p.rows - 1) * p.x_stride + p.k));
   const float* ws = p.ws + n0 / kBlock * p.ws_row;
-  uint32_t x_off[TM];
-  const float* xs[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int row = i * 16 + lr;
-    x_off[i] = row < p.rows ? (uint32_t)(row * (int)p.x_stride + lq * 16) : kOutOfRange;
-    xs[i] = FLOATS ? nullptr : p.xs + (row < p.rows ? row : 0) * p.xs_row;
-  }
-  f32x4 acc[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t x_off = lr < p.rows ? (uint32_t)(lr * (int)p.x_stride + lq * 16) : kOutOfRange;
+  const float* xs = FLOATS ? nullptr : p.xs + (lr < p.rows ? lr : 0) * p.xs_row;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 
   // a piece past k (its 16 bytes all are) reads zeros, blocks past the last one too
   auto load16 = [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int at) __attribute__((always_inline)) {
@@ -616,69 +607,58 @@ __global__ void __launch_bounds__(64 * NW) block_fp8_few_rows_kernel(const GemmP
         i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at + lq * 16 < p.k ? off : kOutOfRange, at, 0));
   };
   for (int kt0 = wave; kt0 < p.blocks; kt0 += NW * UNROLL) {
-    i32x4 wv[UNROLL][2], xv[UNROLL][TM][2];
-    RowPiece<XT> xf[FLOATS ? UNROLL : 1][TM];
-    float sw[UNROLL], sx[UNROLL][TM];
+    i32x4 wv[UNROLL][2], xv[UNROLL][2];
+    RowPiece<XT> xf[FLOATS ? UNROLL : 1];
+    float sw[UNROLL], sx[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int kt = kt0 + u * NW, kb = kt * kBlock;
       wv[u][0] = load16(wr, w_off, kb);
       wv[u][1] = load16(wr, w_off, kb + 64);
       sw[u] = kt < p.blocks ? ws[kt] : 0.f;
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        if constexpr (FLOATS) {
-          const int row = i * 16 + lr;
-          const XT* src = reinterpret_cast<const XT*>(p.x) + row * p.x_stride + kb + lq * 16;
-          load_piece(src, row < p.rows ? p.x_features - kb - lq * 16 : 0, &xf[u][i]);
-        } else {
-          xv[u][i][0] = load16(xr, x_off[i], kb);
-          xv[u][i][1] = load16(xr, x_off[i], kb + 64);
-          sx[u][i] = kt < p.blocks ? xs[i][kt * p.xs_block] : 0.f;
-        }
+      if constexpr (FLOATS) {
+        const XT* src = reinterpret_cast<const XT*>(p.x) + lr * p.x_stride + kb + lq * 16;
+        load_piece(src, lr < p.rows ? p.x_features - kb - lq * 16 : 0, &xf[u]);
+      } else {
+        xv[u][0] = load16(xr, x_off, kb);
+        xv[u][1] = load16(xr, x_off, kb + 64);
+        sx[u] = kt < p.blocks ? xs[kt * p.xs_block] : 0.f;
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const Operand<EXACT> b(__builtin_shufflevector(wv[u][0], wv[u][1], 0, 1, 2, 3, 4, 5, 6, 7));
+      i32x8 bytes;
+      if constexpr (FLOATS)
+        bytes = quantize_piece(xf[u], &sx[u]);
+      else
+        bytes = __builtin_shufflevector(xv[u][0], xv[u][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      const f32x4 part = block_product(b, Operand<EXACT>(bytes));
+      const float s = sx[u] * sw[u];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        i32x8 bytes;
-        if constexpr (FLOATS)
-          bytes = quantize_piece(xf[u][i], &sx[u][i]);
-        else
-          bytes = __builtin_shufflevector(xv[u][i][0], xv[u][i][1], 0, 1, 2, 3, 4, 5, 6, 7);
-        const f32x4 part = block_product(b, Operand<EXACT>(bytes));
-        const float s = sx[u][i] * sw[u];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(part[e], s, acc[i][e]);
-      }
+      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(part[e], s, acc[e]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < TM; ++i) sums[wave][i][lane] = acc[i];
+  sums[wave][lane] = acc;
   __syncthreads();
-  // tile i by wave i % NW, its NW sums in order
+  // the first wave joins the NW sums in order
+  if (wave != 0) return;
+  f32x4 v = sums[0][lane];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    if (i % NW != wave) continue;
-    f32x4 v = sums[0][i][lane];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) v += sums[w][i][lane];
-    const int64_t col = n0 + lq * 4;
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias) load_values(p.bias + col, p.n - col, b);
-    store_columns<EXACT>(p, i * 16 + lr, col, v, b);
-  }
+  for (int w = 1; w < NW; ++w) v += sums[w][lane];
+  const int64_t col = n0 + lq * 4;
+  float b[4] = {0.f, 0.f, 0.f, 0.f};
+  if (p.bias) load_values(p.bias + col, p.n - col, b);
+  store_columns<EXACT>(p, lr, col, v, b);
 }
 
-template <int NW, int TM, int UNROLL, bool EXACT, typename XT>
+template <int NW, int UNROLL, bool EXACT, typename XT>
 int launch_few_rows(GemmParams p, hipStream_t stream) {
   if (p.rows * p.x_stride >= (int64_t)kOutOfRange || 16 * p.w_stride >= (int64_t)kOutOfRange ||
       (p.n + 15) / 16 > 0x7fffffffLL)
     return OMNI_ERR_UNSUPPORTED;
   p.col_tiles = (int)((p.n + 15) / 16);
-  hipLaunchKernelGGL((block_fp8_few_rows_kernel<NW, TM, UNROLL, EXACT, XT>),
+  hipLaunchKernelGGL((block_fp8_few_rows_kernel<NW, UNROLL, EXACT, XT>),
                      dim3((unsigned)p.col_tiles), dim3(64 * NW), 0, stream, p);
   OMNI_LAUNCH_CHECK();
   return OMNI_OK;
@@ -791,7 +771,8 @@ int launch_tile(int tile, const GemmParams& p, hipStream_t s) {
     case kTile64x64:
       // exact products widen each operand: fewer waves with larger parts widen fewer (0.47 us a block
       // against 0.54 on 8 waves; 8-bit products 0.37 on 8, 0.42 on 4)
-      return EXACT ? launch_ring<2, 2, 2, 2, 4, 2, EXACT>(p, s) : launch_ring<2, 4, 2, 1, 4, 2, EXACT>(p, s);
+      if constexpr (EXACT) return launch_ring<2, 2, 2, 2, 4, 2, true>(p, s);
+      else return launch_ring<2, 4, 2, 1, 4, 2, false>(p, s);
     case kTile64x128: return launch_ring<2, 4, 2, 2, 3, 2, EXACT>(p, s);
     case kTile128x128: return launch_gemm<2, 2, 4, 4, EXACT>(p, s);
     default: break;
@@ -806,10 +787,10 @@ int launch_tile(int tile, const GemmParams& p, hipStream_t s) {
 template <bool EXACT>
 int launch_few(int x_dtype, const GemmParams& p, hipStream_t s) {
   switch (x_dtype) {
-    case OMNI_DTYPE_FP8_E4M3: return launch_few_rows<8, 1, 2, EXACT, uint8_t>(p, s);
-    case OMNI_DTYPE_F32: return launch_few_rows<16, 1, 1, EXACT, float>(p, s);
-    case OMNI_DTYPE_BF16: return launch_few_rows<16, 1, 1, EXACT, __bf16>(p, s);
-    default: return launch_few_rows<16, 1, 1, EXACT, _Float16>(p, s);
+    case OMNI_DTYPE_FP8_E4M3: return launch_few_rows<8, 2, EXACT, uint8_t>(p, s);
+    case OMNI_DTYPE_F32: return launch_few_rows<16, 1, EXACT, float>(p, s);
+    case OMNI_DTYPE_BF16: return launch_few_rows<16, 1, EXACT, __bf16>(p, s);
+    default: return launch_few_rows<16, 1, EXACT, _Float16>(p, s);
   }
 }
 
