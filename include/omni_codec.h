@@ -770,6 +770,9 @@ int omni_block_quantize(const void* x, int x_dtype, int64_t x_stride, int64_t ro
  * does, up to OMNI_BLOCK_FP8_FEW_ROWS rows inside the product's launch, more of them in a launch
  * before it into workspace (16-byte aligned, at least rows * (k + 4 * ceil(k / 128)) bytes).
  *
+ * An element's K blocks are added in ascending order whatever the row count, so a row's bits do not
+ * depend on the rows beside it, and float rows give the bits of those rows quantized before.
+ *
  * bf16 outputs multiply on the 8-bit matrix cores, which cut each product below 2^-13 of the
  * largest of the 8 it is added with (up to 5e-5 of a result); f16 and f32 outputs on the bf16 ones,
  * where the sums are float32 throughout.

@@ -31,6 +31,7 @@ struct GemmParams {
   int64_t out_stride;
   int out_dtype;
   int row_tiles, col_tiles;
+  int chunk;  // few rows: K blocks whose products are in LDS at a time
 };
 
 // Four consecutive columns of one row, rounded once to the output's type.
@@ -532,9 +533,11 @@ int launch_ring(GemmParams p, hipStream_t stream) {
 // ------------------------------------------------------------------------------ few rows
 //
 // Up to 16 rows: the weight's bytes are the time, each read once. A workgroup takes 16 columns of all
-// rows; its waves take K blocks in turn and load their operands straight into MFMA registers, UNROLL blocks of them in flight, no LDS and no barrier until the waves' sums meet. x is
-// E4M3 rows, or (XT) float rows, whose groups each wave quantizes for itself: the bits of
-// omni_block_quantize without its launch.
+// rows; its waves take K blocks in turn and load their operands straight into MFMA registers, UNROLL
+// blocks of them in flight. The blocks' products meet in LDS and are added in the blocks' order, as
+// every other tile adds them, so that a row's bits are the same in any batch (a sum per wave, joined
+// at the end, took 0.1 us less at 8 blocks and 0.8 us less at 64). x is E4M3 rows, or (XT) float rows,
+// whose groups each wave quantizes for itself: the bits of omni_block_quantize without its launch.
 
 // What a lane holds of a row's K block: bytes (values) 16 q .. 16 q + 15 and 64 + 16 q .. + 15.
 template <typename XT>
@@ -584,10 +587,17 @@ OMNI_DEVICE i32x8 quantize_piece(const RowPiece<XT>& piece, float* scale) {
   return bytes;
 }
 
+// LDS bytes of a K block's products and scales, and how many blocks' a workgroup takes at most: two
+// workgroups a CU then.
+constexpr int kFewBlockBytes = 1024 + 64, kFewChunk = 64;
+
 template <int NW, int UNROLL, bool EXACT, typename XT>
 __global__ void __launch_bounds__(64 * NW) block_fp8_few_rows_kernel(const GemmParams p) {
   constexpr bool FLOATS = !std::is_same<XT, uint8_t>::value;
-  __shared__ f32x4 sums[NW][64];
+  static_assert(NW >= 8, "a wave for each block that fills up eight");
+  extern __shared__ __attribute__((aligned(16))) f32x4 products[];     // [chunk][64 lanes]
+  float* scales = reinterpret_cast<float*>(products + p.chunk * 64);  // [chunk][16 rows]
+  const int rows = (int)p.rows;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
@@ -597,59 +607,78 @@ __global__ void __launch_bounds__(64 * NW) block_fp8_few_rows_kernel(const GemmP
   const uint32_t w_off = lr < n_rows ? (uint32_t)(lr * (int)p.w_stride + lq * 16) : kOutOfRange;
   const auto xr = buffer_rsrc(p.x, FLOATS ? 0u : (uint32_t)((p.rows - 1) * p.x_stride + p.k));
   const float* ws = p.ws + n0 / kBlock * p.ws_row;
-  const uint32_t x_off = lr < p.rows ? (uint32_t)(lr * (int)p.x_stride + lq * 16) : kOutOfRange;
-  const float* xs = FLOATS ? nullptr : p.xs + (lr < p.rows ? lr : 0) * p.xs_row;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t x_off = lr < rows ? (uint32_t)(lr * (int)p.x_stride + lq * 16) : kOutOfRange;
+  const float* xs = FLOATS ? nullptr : p.xs + (lr < rows ? lr : 0) * p.xs_row;
 
   // a piece past k (its 16 bytes all are) reads zeros, blocks past the last one too
   auto load16 = [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int at) __attribute__((always_inline)) {
     return __builtin_bit_cast(
         i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at + lq * 16 < p.k ? off : kOutOfRange, at, 0));
   };
-  for (int kt0 = wave; kt0 < p.blocks; kt0 += NW * UNROLL) {
-    i32x4 wv[UNROLL][2], xv[UNROLL][2];
-    RowPiece<XT> xf[FLOATS ? UNROLL : 1];
-    float sw[UNROLL], sx[UNROLL];
+  // the sums: element threadIdx.x % 4 of lane threadIdx.x / 4, in the first four waves
+  const int out_row = threadIdx.x >> 2 & 15;
+  const int64_t col = n0 + (threadIdx.x >> 6) * 4 + (threadIdx.x & 3);
+  float acc = 0.f;
+  for (int c0 = 0; c0 < p.blocks; c0 += p.chunk) {
+    const int held = p.blocks - c0 < p.chunk ? p.blocks - c0 : p.chunk;
+    if (c0 > 0) __syncthreads();  // the products before these are added
+    if (const int at = held + wave; at < (held + 7) / 8 * 8) {  // the sums take eight blocks at a time
+      products[at * 64 + lane] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (lane < 16) scales[at * 16 + lane] = 0.f;
+    }
+    for (int at0 = wave; at0 < held; at0 += NW * UNROLL) {
+      i32x4 wv[UNROLL][2], xv[UNROLL][2];
+      RowPiece<XT> xf[FLOATS ? UNROLL : 1];
+      float sw[UNROLL], sx[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int kt = kt0 + u * NW, kb = kt * kBlock;
-      wv[u][0] = load16(wr, w_off, kb);
-      wv[u][1] = load16(wr, w_off, kb + 64);
-      sw[u] = kt < p.blocks ? ws[kt] : 0.f;
-      if constexpr (FLOATS) {
-        const XT* src = reinterpret_cast<const XT*>(p.x) + lr * p.x_stride + kb + lq * 16;
-        load_piece(src, lr < p.rows ? p.x_features - kb - lq * 16 : 0, &xf[u]);
-      } else {
-        xv[u][0] = load16(xr, x_off, kb);
-        xv[u][1] = load16(xr, x_off, kb + 64);
-        sx[u] = kt < p.blocks ? xs[kt * p.xs_block] : 0.f;
+      for (int u = 0; u < UNROLL; ++u) {
+        const int kt = c0 + at0 + u * NW, kb = kt * kBlock;
+        wv[u][0] = load16(wr, w_off, kb);
+        wv[u][1] = load16(wr, w_off, kb + 64);
+        sw[u] = kt < p.blocks ? ws[kt] : 0.f;
+        if constexpr (FLOATS) {
+          const XT* src = reinterpret_cast<const XT*>(p.x) + lr * p.x_stride + kb + lq * 16;
+          load_piece(src, lr < rows ? p.x_features - kb - lq * 16 : 0, &xf[u]);
+        } else {
+          xv[u][0] = load16(xr, x_off, kb);
+          xv[u][1] = load16(xr, x_off, kb + 64);
+          sx[u] = kt < p.blocks ? xs[kt * p.xs_block] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const Operand<EXACT> b(__builtin_shufflevector(wv[u][0], wv[u][1], 0, 1, 2, 3, 4, 5, 6, 7));
+        i32x8 bytes;
+        if constexpr (FLOATS)
+          bytes = quantize_piece(xf[u], &sx[u]);
+        else
+          bytes = __builtin_shufflevector(xv[u][0], xv[u][1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const f32x4 part = block_product(b, Operand<EXACT>(bytes));
+        const int at = at0 + u * NW;
+        if (u == 0 || at < held) {
+          products[at * 64 + lane] = part;
+          if (lq == 0) scales[at * 16 + lr] = sx[u] * sw[u];
+        }
       }
     }
+    __syncthreads();
+    if (wave < 4) {
+      const float* part = reinterpret_cast<const float*>(products) + threadIdx.x;
+      const float* s = scales + out_row;
+      for (int j0 = 0; j0 < held; j0 += 8, part += 8 * 256, s += 8 * 16)
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const Operand<EXACT> b(__builtin_shufflevector(wv[u][0], wv[u][1], 0, 1, 2, 3, 4, 5, 6, 7));
-      i32x8 bytes;
-      if constexpr (FLOATS)
-        bytes = quantize_piece(xf[u], &sx[u]);
-      else
-        bytes = __builtin_shufflevector(xv[u][0], xv[u][1], 0, 1, 2, 3, 4, 5, 6, 7);
-      const f32x4 part = block_product(b, Operand<EXACT>(bytes));
-      const float s = sx[u] * sw[u];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(part[e], s, acc[e]);
+        for (int j = 0; j < 8; ++j) acc = __builtin_fmaf(part[j * 256], s[j * 16], acc);
     }
   }
-  sums[wave][lane] = acc;
-  __syncthreads();
-  // the first wave joins the NW sums in order
-  if (wave != 0) return;
-  f32x4 v = sums[0][lane];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) v += sums[w][lane];
-  const int64_t col = n0 + lq * 4;
-  float b[4] = {0.f, 0.f, 0.f, 0.f};
-  if (p.bias) load_values(p.bias + col, p.n - col, b);
-  store_columns<EXACT>(p, lr, col, v, b);
+  if (wave >= 4 || out_row >= rows || col >= p.n) return;
+  const float v[1] = {acc + (p.bias ? p.bias[col] : 0.f)};
+  const int64_t at = out_row * p.out_stride + col;
+  if (!EXACT)
+    store_values<__bf16, 1>(static_cast<__bf16*>(p.out) + at, 1, v);
+  else if (p.out_dtype == OMNI_DTYPE_F32)
+    store_values<float, 1>(static_cast<float*>(p.out) + at, 1, v);
+  else
+    store_values<_Float16, 1>(static_cast<_Float16*>(p.out) + at, 1, v);
 }
 
 template <int NW, int UNROLL, bool EXACT, typename XT>
@@ -657,9 +686,16 @@ int launch_few_rows(GemmParams p, hipStream_t stream) {
   if (p.rows * p.x_stride >= (int64_t)kOutOfRange || 16 * p.w_stride >= (int64_t)kOutOfRange ||
       (p.n + 15) / 16 > 0x7fffffffLL)
     return OMNI_ERR_UNSUPPORTED;
+  const int all = (p.blocks + 7) / 8 * 8;
+  p.chunk = all < kFewChunk ? all : kFewChunk;
   p.col_tiles = (int)((p.n + 15) / 16);
-  hipLaunchKernelGGL((block_fp8_few_rows_kernel<NW, UNROLL, EXACT, XT>),
-                     dim3((unsigned)p.col_tiles), dim3(64 * NW), 0, stream, p);
+  auto k = block_fp8_few_rows_kernel<NW, UNROLL, EXACT, XT>;
+  static const bool raised = hipFuncSetAttribute((const void*)k,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kFewChunk * kFewBlockBytes) == hipSuccess;
+  if (!raised) return OMNI_ERR_LAUNCH;
+  hipLaunchKernelGGL(k, dim3((unsigned)p.col_tiles), dim3(64 * NW),
+                     (unsigned)(p.chunk * kFewBlockBytes), stream, p);
   OMNI_LAUNCH_CHECK();
   return OMNI_OK;
 }
@@ -782,8 +818,8 @@ int launch_tile(int tile, const GemmParams& p, hipStream_t s) {
 }
 
 // Up to 16 rows: 8 waves of two blocks in flight each, or, quantizing float rows themselves, 16 of
-// one (1 x 1024 -> 2048 3.3 us, 16 x 4096 -> 4096 7.5 us; 4 or 16 waves within 0.6 us; float rows
-// 4.7 and 8.9 us, with 8 waves 6.0 and 11.3, and 2 - 3 us more launched apart).
+// one (1 x 1024 -> 2048 3.5 us, 16 x 4096 -> 4096 8.2; 16 waves of one block 3.4 and 8.7; float rows
+// 4.1 and 8.6, with 8 waves 4.1 and 10.4, quantized by a launch before 5.6 and 11.2).
 template <bool EXACT>
 int launch_few(int x_dtype, const GemmParams& p, hipStream_t s) {
   switch (x_dtype) {

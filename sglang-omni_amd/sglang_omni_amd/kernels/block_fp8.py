@@ -107,7 +107,8 @@ def block_fp8_linear(x: torch.Tensor | BlockFp8Rows, weight: BlockFp8Weight,
                      out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """out = x @ W^T + bias [rows, out_features] on the current stream, float32 sums rounded once to
     out_dtype (bf16, f16 or f32; ``out``'s own when it is given). x is ``BlockFp8Rows``, or a float
-    tensor [rows, features] that is quantized as ``quantize_block_rows`` does. bf16 outputs multiply
+    tensor [rows, features] that is quantized as ``quantize_block_rows`` does, to the same bits. A row's
+    bits do not depend on the rows beside it. bf16 outputs multiply
     on the 8-bit matrix cores (up to 5e-5 of a result off); f16 and f32 ones on the bf16 matrix
     cores, exact products in float32 sums, at about half the rate."""
     w, w_scale, bias = weight.weight, weight.scale, weight.bias
