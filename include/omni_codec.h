@@ -763,7 +763,9 @@ int omni_block_quantize(const void* x, int x_dtype, int64_t x_stride, int64_t ro
  * (bf16, f16 or f32). x [rows][k] and w [n][k] E4M3, 16-byte aligned, rows x_stride / w_stride
  * bytes apart (multiples of 16), k a multiple of 16 up to 2^20; x_scale at m * x_scale_stride_row
  * + b * x_scale_stride_block; w_scale rows w_scale_stride apart. out rows out_stride elements
- * apart, any alignment of its type, and no input. rows = 0 does nothing.
+ * apart, any alignment of its type, and no input. rows = 0 does nothing. Strides with which the
+ * 8-bit rows of a tile (up to 256 of x, 256 of w) or their scales span 2 GiB are
+ * OMNI_ERR_UNSUPPORTED.
  *
  * x may be bf16 / f16 / f32 rows instead (x_dtype, x_stride in elements, any alignment of the type;
  * `features` of them, which rounded up to 16 make k): they are quantized as omni_block_quantize

@@ -683,8 +683,10 @@ __global__ void __launch_bounds__(64 * NW) block_fp8_few_rows_kernel(const GemmP
 
 template <int NW, int UNROLL, bool EXACT, typename XT>
 int launch_few_rows(GemmParams p, hipStream_t stream) {
-  if (p.rows * p.x_stride >= (int64_t)kOutOfRange || 16 * p.w_stride >= (int64_t)kOutOfRange ||
-      (p.n + 15) / 16 > 0x7fffffffLL)
+  // 8-bit rows are read through a buffer resource, float rows by their addresses
+  constexpr bool FLOATS = !std::is_same<XT, uint8_t>::value;
+  if ((!FLOATS && p.rows * p.x_stride >= (int64_t)kOutOfRange) ||
+      16 * p.w_stride >= (int64_t)kOutOfRange || (p.n + 15) / 16 > 0x7fffffffLL)
     return OMNI_ERR_UNSUPPORTED;
   const int all = (p.blocks + 7) / 8 * 8;
   p.chunk = all < kFewChunk ? all : kFewChunk;
