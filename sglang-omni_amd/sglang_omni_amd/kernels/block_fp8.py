@@ -105,12 +105,15 @@ def quantize_block_rows(x: torch.Tensor) -> BlockFp8Rows:
 def block_fp8_linear(x: torch.Tensor | BlockFp8Rows, weight: BlockFp8Weight,
                      out: torch.Tensor | None = None, *,
                      out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """out = x @ W^T + bias [rows, out_features] on the current stream, float32 sums rounded once to
-    out_dtype (bf16, f16 or f32; ``out``'s own when it is given). x is ``BlockFp8Rows``, or a float
-    tensor [rows, features] that is quantized as ``quantize_block_rows`` does, to the same bits. A row's
-    bits do not depend on the rows beside it. bf16 outputs multiply
-    on the 8-bit matrix cores (up to 5e-5 of a result off); f16 and f32 ones on the bf16 matrix
-    cores, exact products in float32 sums, at about half the rate."""
+    """out = x @ W^T + bias [rows, out_features] on the current stream, summed in float32 and rounded
+    once to out_dtype (bf16, f16 or f32; ``out``'s own when it is given). x is ``BlockFp8Rows``, or a float
+    tensor [rows, features] that is quantized as ``quantize_block_rows`` does, to the same bits. A
+    row's bits do not depend on the rows beside it.
+
+    bf16 outputs multiply on the 8-bit matrix cores, which lose up to 7 * 2^-13 of the largest product
+    of each 8 features (far less than the bf16 rounding, unless larger products cancel); f16 and f32
+    ones on the bf16 matrix cores, exact products in float32 sums, at about half the rate: a bf16
+    result of float32 sums is ``out_dtype=torch.float32`` and a cast."""
     w, w_scale, bias = weight.weight, weight.scale, weight.bias
     if type(x) is BlockFp8Rows:
         values, scale = x.values, x.scale
