@@ -57,7 +57,7 @@ class Layer:
 
 
 class Talker:
-    """The weights, and for `slots` streams the K / V rings, positions and token histories."""
+    """The weights, and for `slots` streams the K / V rings, positions and the last `history` tokens."""
 
     def __init__(self, config: TalkerConfig, slots: int, device: torch.device, seed: int = 0,
                  history: int = 4096):
@@ -144,7 +144,9 @@ class Talker:
                       allowed=self.allowed, allowed_index=torch.full_like(slot_index, codebook),
                       out=logits)
         nxt = logits.argmax(1)
-        self.history[slot_index, self.lengths[slot_index].long()] = nxt.to(torch.int32)
+        # the history is a ring: the penalties are those of a stream's last tokens
+        at = self.lengths[slot_index].long() % self.history.shape[1]
+        self.history[slot_index, at] = nxt.to(torch.int32)
         self.lengths[slot_index] += 1
         return nxt
 
