@@ -900,7 +900,7 @@ int omni_rotary(const omni_rotary_args* args, omni_stream_t stream);
  * [masks][ceil(vocab / 32)] int32, token v at bit v % 32 of word v / 32, rows allowed_stride
  * apart; row r reads mask allowed_index[r] (or r), none where that is out of range. A row whose
  * mask allows nothing is all -infinity. out may be logits (same type and stride). vocab up to
- * 2^30; rows = 0 does nothing.
+ * 2^30, capacity below it; rows = 0 does nothing.
  */
 typedef struct omni_logits_args {
   const void* logits;

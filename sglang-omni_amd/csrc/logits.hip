@@ -44,6 +44,7 @@ struct Word {
   }
 };
 constexpr int64_t kNarrowHistory = 1 << 14;
+constexpr int64_t kMaxHistory = (1 << 30) - 1;  // tokens: kMade of the wide words
 
 struct LogitParams {
   const void* logits;
@@ -275,7 +276,8 @@ extern "C" int omni_adjust_logits(const omni_logits_args* a, omni_stream_t strea
       !aligned_to(a->logits, size(a->dtype)) || !aligned_to(a->out, size(a->out_dtype)))
     return OMNI_ERR_INVALID_ARG;
   const int token_size = a->tokens_dtype == OMNI_DTYPE_I64 ? 8 : 4;
-  if (a->history && (!a->lengths || a->capacity < 0 || a->capacity > 0x40000000LL || a->history_stride < a->capacity ||
+  if (a->history && (!a->lengths || a->capacity < 0 || a->capacity > kMaxHistory ||
+                     a->history_stride < a->capacity ||
                      a->slots < 1 || (!a->slot_index && a->slots < a->rows) ||
                      !aligned_to(a->history, token_size)))
     return OMNI_ERR_INVALID_ARG;

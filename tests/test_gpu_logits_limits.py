@@ -1,0 +1,22 @@
+"""Limits of the logit adjustments: the largest history."""
+
+from __future__ import annotations
+
+from sglang_omni_amd import _native as N
+
+
+def test_counts_fit_their_words():
+    """A token's count has 30 bits, so 2^30 tokens of history are refused. Without a GPU: the rows
+    (2^31) are past what a launch takes, so 2^30 - 1 tokens are refused as unsupported instead."""
+    fields = [name for name, _ in N.LogitsArgs._fields_]
+
+    def status(capacity):
+        values = dict.fromkeys(fields, 0)
+        values |= {name: 4096 for name in ("logits", "out", "history", "lengths")}
+        values |= {"dtype": N.DTYPE_F32, "out_dtype": N.DTYPE_F32, "tokens_dtype": N.DTYPE_I32,
+                   "lengths_dtype": N.DTYPE_I32, "logits_stride": 64, "out_stride": 64, "vocab": 64,
+                   "rows": 2**31, "slots": 2**31, "history_stride": capacity, "capacity": capacity}
+        return N.load_library().omni_adjust_logits(N.pack_logits(*values.values()), None)
+
+    assert status(2**30 - 1) == N.UNSUPPORTED
+    assert status(2**30) == N.INVALID_ARG
