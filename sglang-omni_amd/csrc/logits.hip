@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, 8) adjust_logits_kernel(const LogitP
       const int64_t first = p.prompt_lengths ? load_index(p.prompt_lengths, p.lengths64, slot) : 0;
       length = (int)(held < p.capacity ? held : p.capacity);
       length = held < 0 ? 0 : length;
-      prompt = (int)(first < length ? first : length);
+      prompt = first < 0 ? 0 : (int)(first < length ? first : length);
       tokens = static_cast<const H*>(p.history) + slot * p.history_stride;
     }
   }
