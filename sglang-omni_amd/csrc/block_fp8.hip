@@ -195,6 +195,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) block_fp8_gemm_kernel(const G
   const int s_part = wave % T::SCALE_PARTS;
   const int s_row = s_part * 64 + lane;
   const uint32_t s_off = s_row < m_rows ? (uint32_t)(s_row * (int)p.xs_row) * 4u : kOutOfRange;
+  const int s_step = (int)p.xs_block * 4;
   // DMA instruction c of block kt: w's pieces and the scales, x's first half, x's second half. The
   // last block may end early, and blocks past it are empty: their pieces read zeros.
   auto issue = [&](int kt, int c) __attribute__((always_inline)) {
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) block_fp8_gemm_kernel(const G
     } else if (c == T::B_PER_WAVE) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           sr, (__attribute__((address_space(3))) void*)(st + s_part * 256), 4,
-          (int)(kt < p.blocks ? s_off : kOutOfRange), kt * (int)p.xs_block * 4, 0, 0);
+          (int)(kt < p.blocks ? s_off : kOutOfRange), min(kt, p.blocks - 1) * s_step, 0, 0);
     } else {
       const int a = c - T::B_PER_WAVE - 1, half = a / T::A_HALF, piece = a % T::A_HALF;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(64 * WM * WN) block_fp8_ring_kernel(const Gemm
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           sr, (__attribute__((address_space(3))) void*)(st + part * 256), 4,
           (int)(stage * G + s_block[i] < p.blocks ? s_off[i] : kOutOfRange),
-          stage * G * (int)p.xs_block * 4, 0, 0);
+          stage * G < p.blocks ? stage * G * (int)p.xs_block * 4 : 0, 0, 0);
     }
   };
   const int lr = lane & 15, lq = lane >> 4;
@@ -895,7 +896,7 @@ extern "C" int omni_block_fp8_gemm(const omni_block_fp8_args* a, omni_stream_t s
   const bool exact = a->out_dtype != OMNI_DTYPE_BF16;
   if (few)
     return exact ? launch_few<true>(a->x_dtype, p, s) : launch_few<false>(a->x_dtype, p, s);
-  // the DMAs address a tile's scales with 32-bit byte offsets
+  // the DMAs address a tile's scales, up to those of the last block, with 32-bit byte offsets
   if (256 * p.xs_row + blocks * p.xs_block >= 0x1fffffffLL) return OMNI_ERR_UNSUPPORTED;
   if (floats) {
     uint8_t* q = static_cast<uint8_t*>(a->workspace);
