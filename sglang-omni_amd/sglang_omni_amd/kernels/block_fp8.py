@@ -49,8 +49,9 @@ class BlockFp8Rows:
 
 def pack_block_fp8(weight: torch.Tensor, bias: torch.Tensor | None = None) -> BlockFp8Weight:
     """weight [out, in] (any float dtype) -> E4M3 with a scale per block of 128 x 128, scale =
-    max|block| / 448 (1 for a block of zeros). Inputs short of a multiple of 16 are filled up with
-    zero weights, as ``quantize_block_rows`` fills its rows."""
+    max|block| / 448 (1 for a block of zeros). NaN stays NaN and leaves the scale to the others; an
+    infinity makes it infinite, so that every product with the block is NaN. Inputs short of a
+    multiple of 16 are filled up with zero weights, as ``quantize_block_rows`` fills its rows."""
     if weight.dim() != 2:
         raise ValueError("a linear weight is [out_features, in_features]")
     n, k = weight.shape
@@ -58,7 +59,7 @@ def pack_block_fp8(weight: torch.Tensor, bias: torch.Tensor | None = None) -> Bl
     w = torch.zeros(rb * BLOCK, cb * BLOCK, dtype=torch.float32, device=weight.device)
     w[:n, :k] = weight.detach().float()
     w = w.view(rb, BLOCK, cb, BLOCK)
-    amax = w.abs().amax((1, 3), keepdim=True)
+    amax = w.abs().nan_to_num(0.0, posinf=float("inf")).amax((1, 3), keepdim=True)
     scale = torch.where(amax >= 2.0 ** -100, amax / 448.0, torch.ones_like(amax))
     q = (w / scale).to(_E4M3).view(rb * BLOCK, cb * BLOCK)[:n, :-(-k // 16) * 16]
     return BlockFp8Weight(q.contiguous(), scale.view(rb, cb).contiguous(),
