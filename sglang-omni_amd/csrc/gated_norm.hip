@@ -11,6 +11,9 @@
 // registers of the 64, 256 or 1024 threads that hold it, 8 to 32 channels each, in float32; variances
 // are sums of squared differences from the mean, formed after it. 16384 x 4096 in bf16, both norms, a
 // gate per token: 127 us, 5.3 TB/s. Rows of up to 1024 channels are a wave's, without a barrier.
+// With fewer rows, which do not hide it, the latency of a wave's own loads bounds it (3003 x 1000 10.5
+// us, 2.4 TB/s; 1 x 1024 5.2 us): those of y and x stand under load_values' branches, each complete
+// before the next goes out, and the weights, biases and the gate are loaded after the sums.
 #include <type_traits>
 
 #include "block_fp8.h"

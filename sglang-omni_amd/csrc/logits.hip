@@ -11,10 +11,14 @@
 //
 // A workgroup takes a tile of a row's vocabulary. The dense part of the work, the mask, streams
 // through it and looks at nothing else. The history's tokens that fall into the tile are counted in
-// LDS meanwhile (integer atomics, whose order changes nothing); whoever finds a token's word empty
+// LDS (integer atomics, whose order changes nothing); whoever finds a token's word empty
 // puts it on a list, and the listed tokens and bias entries, few beside the tile, are computed one to
 // a thread and stored over the dense part's values. (Looking every logit's count up instead took 20 instructions
 // a logit: 200 x 50257 in bf16 16.7 us, 64 x 131072 in float32 with everything 25.9.)
+//
+// HBM would bound it (64 x 131072 in float32 13.7 us); what does is a workgroup's chain, of which a call
+// of one round of workgroups hides nothing: lengths, tokens and bias entries, then the logits and mask
+// words, then the counts, then the values (23.7 us; the mask alone 12.8, with histories 17.8).
 #include <type_traits>
 
 #include "block_fp8.h"
@@ -105,8 +109,9 @@ __global__ void __launch_bounds__(kThreads, 8) adjust_logits_kernel(const LogitP
   const int64_t tile_tokens = p.vocab - v0 < kTile ? p.vocab - v0 : kTile;
   const H* biased = static_cast<const H*>(p.bias_tokens) + row * p.bias_tokens_stride;
   const float* bias_values = p.bias_values + row * p.bias_values_stride;
-  // 16-byte loads, all of a round's before the first is used. The first round goes out ahead of the
-  // logits: loads complete in order, so it is counted while they are still coming.
+  // 16-byte loads, all of a round's before the first is used; the first round goes out ahead of the
+  // logits. It is counted after they have come, though: each mask word below is waited for under its
+  // branch, and with it all that went out before.
   constexpr int PER_LOAD = 16 / sizeof(H), LOADS = 2, ROUND = kThreads * PER_LOAD * LOADS;
   H held[LOADS][PER_LOAD];
   auto load_round = [&](int base) __attribute__((always_inline)) {
@@ -131,7 +136,8 @@ __global__ void __launch_bounds__(kThreads, 8) adjust_logits_kernel(const LogitP
   const bool has_entry = tid < p.biases;
   const H entry_token = has_entry ? biased[tid] : (H)-1;
   const float entry_value = has_entry ? bias_values[tid] : 0.f;
-  // and 64 entries of the list in each wave's lanes, ids outside the vocabulary as -1
+  // and 64 entries of the list in each wave's lanes, ids outside the vocabulary as -1 (looked at, and so
+  // waited for, before the logits go out)
   auto load_entries = [&](int64_t base) __attribute__((always_inline)) {
     const int64_t i = base + (tid & 63);
     const int64_t token = i < p.biases ? (int64_t)biased[i] : -1;
@@ -221,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, 8) adjust_logits_kernel(const LogitP
     if (c & W::kBiased) t += bias;
     return (O)((word >> (v & 31)) & 1u ? t : -__builtin_huge_valf());
   };
-  // this thread's listed token (unless a bias entry speaks for it) and bias entry, while the dense
-  // part's logits are still coming
+  // this thread's listed token (unless a bias entry speaks for it) and bias entry, ahead of the dense
+  // part's stores
   uint32_t first_at = 0;
   bool first_mine = false;
   O first = (O)0.f, entry = (O)0.f;

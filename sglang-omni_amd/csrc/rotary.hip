@@ -60,9 +60,11 @@ OMNI_DEVICE void sincos_turn(double turn, float* s, float* c) {
 constexpr int kHeadsPerThread = 4;
 
 // A thread turns V pairs of one frequency chunk of up to four heads of a token (or copies 2 V values
-// past the turned ones), so that its sines and cosines serve all four; all of its loads are out before
-// the first sine. HBM bounds it: 16001 tokens of 40 heads of 128 in bf16 74 us, 4.4 TB/s (a copy 5.05);
-// two heads a thread 82 us, eight 76.
+// past the turned ones), so that its sines and cosines serve all four. HBM bounds it where other waves
+// hide a wave's latency: 16001 tokens of 40 heads of 128 in bf16 74 us, 4.4 TB/s (a copy 5.05); two
+// heads a thread 82 us, eight 76. In few tokens its own chain does, 64 of 24 heads 6.2 us: each of the
+// eight loads stands under a branch of load_values, through a pointer that is q's or k's, and is
+// complete before the next goes out; the position and the frequencies follow them.
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
