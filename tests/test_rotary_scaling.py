@@ -1,5 +1,5 @@
 """Rope scalings as configurations write them: every key is honoured or refused, against each
-definition written out for single pairs and against transformers' own (float32, so within 1e-4)."""
+definition written out for single pairs."""
 
 from __future__ import annotations
 
@@ -11,20 +11,6 @@ import torch
 from sglang_omni_amd.kernels import rotary_frequencies
 
 YARN = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
-
-
-def _theirs(dim, base, scaling, context):
-    rope = pytest.importorskip("transformers.modeling_rope_utils")
-    from transformers import PretrainedConfig
-
-    config = PretrainedConfig()
-    config.rope_theta, config.max_position_embeddings = base, context
-    config.head_dim = config.hidden_size = dim
-    config.num_attention_heads = 1
-    config.rope_scaling = dict(scaling)
-    config.rope_parameters = dict(scaling, rope_theta=base)
-    inv, factor = rope.ROPE_INIT_FUNCTIONS[scaling["rope_type"]](config, device="cpu")
-    return inv.double(), factor
 
 
 def _yarn_by_hand(dim, base, factor, original, truncate, fast=32.0, slow=1.0):
@@ -60,9 +46,6 @@ def test_yarn(dim, base, extra, factor):
                          extra.get("beta_fast") or 32.0, extra.get("beta_slow") or 1.0)
     assert torch.allclose(got, want, rtol=1e-12, atol=0)
     assert got_factor == pytest.approx(factor, rel=1e-12)
-    theirs, their_factor = _theirs(dim, base, {**YARN, **extra}, 40 * 4096)
-    assert torch.allclose(got, theirs, rtol=1e-4, atol=0)
-    assert got_factor == pytest.approx(their_factor, rel=1e-6)
 
 
 def test_longrope():
@@ -75,9 +58,7 @@ def test_longrope():
     assert factor == pytest.approx(math.sqrt(1 + math.log(32) / math.log(4096)), rel=1e-12)
     assert torch.allclose(got, plain / torch.tensor([1.0, 2.0, 3.0, 4.0], dtype=torch.float64))
     short, _ = rotary_frequencies(8, 1e4, {**scaling, "factor": 32.0, "short": True})
-    theirs, their_factor = _theirs(8, 1e4, scaling, 32 * 4096)
-    assert factor == pytest.approx(their_factor, rel=1e-6)
-    assert torch.allclose(short, theirs, rtol=1e-4, atol=0)
+    assert torch.allclose(short, plain / torch.tensor([1.0, 1.1, 1.2, 1.3], dtype=torch.float64))
     del scaling["original_max_position_embeddings"]
     _, given = rotary_frequencies(8, 1e4, {**scaling, "attention_factor": 1.25})
     assert given == 1.25
