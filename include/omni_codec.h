@@ -930,6 +930,150 @@ typedef struct omni_logits_args {
 } omni_logits_args;
 int omni_adjust_logits(const omni_logits_args* args, omni_stream_t stream);
 
+/*
+ * A paged key-value cache: rows [pages][kv_heads][page_size][dim] of keys and of values, of one type
+ * (bf16, f16, or E4M3 with a float32 scale per row [pages][kv_heads][page_size]) and of the same
+ * strides, in elements, dim contiguous. A slot is page * page_size + place; pages * page_size is at
+ * most 2^31 - 1. An E4M3 row has scale = max|row| / 448 and holds E4M3(x * (448 / max|row|)), both in
+ * float32, rounded to nearest even; a row whose largest magnitude is below 2^-100 holds zeros with
+ * scale 1. NaN stays NaN; a row with an infinity has an infinite scale.
+ */
+typedef struct omni_kv_cache {
+  void* keys;
+  void* values;
+  int dtype;
+  int64_t stride_page, stride_head, stride_token;
+  float* key_scale;
+  float* value_scale;
+  int64_t scale_stride_page, scale_stride_head, scale_stride_token;
+  int64_t pages, page_size, kv_heads, dim;
+} omni_kv_cache;
+
+/*
+ * omni_norm_rotary: the heads of a layer between its qkv product and its attention, q [tokens][heads]
+ * [dim], k and v [tokens][kv_heads][dim] of one type (bf16, f16, f32), token and head strides free, dim
+ * contiguous, any alignment of the type:
+ *
+ *   normed: q and k heads x / sqrt(mean(x^2) + eps) * weight   (weights float32 [dim], each optional)
+ *   pairs > 0: their first 2 * pairs values turned as omni_rotary does
+ *   cache: k (after both) and v into the rows of slots[token] (int32 / int64); a token whose slot is
+ *     not in the cache, a negative one for instance, writes no row. Tokens of one call need slots of
+ *     their own: what two tokens write to one row is any mix of both.
+ *
+ * float32 throughout, rounded once to the type; the cache gets the rounded values. heads may be 0, and
+ * k_out null where only the cache takes k; v is read with a cache only. q_out may be q and k_out k
+ * (same strides), else nothing overlaps. dim up to 512 (else OMNI_ERR_UNSUPPORTED); tokens = 0 does
+ * nothing.
+ */
+typedef struct omni_norm_rotary_args {
+  const void* q;
+  int64_t q_stride_token, q_stride_head;
+  const void* k;
+  int64_t k_stride_token, k_stride_head;
+  const void* v;
+  int64_t v_stride_token, v_stride_head;
+  void* q_out;
+  int64_t q_out_stride_token, q_out_stride_head;
+  void* k_out;
+  int64_t k_out_stride_token, k_out_stride_head;
+  int dtype;
+  int64_t tokens, heads, kv_heads, dim;
+  int normed;
+  const float* q_weight;
+  const float* k_weight;
+  float eps;
+  int64_t pairs;
+  const void* positions;
+  int positions_dtype;
+  int64_t positions_stride;
+  const double* inv_freq;
+  float factor;
+  int layout;
+  const omni_kv_cache* cache;
+  const void* slots;
+  int slots_dtype;
+  int64_t slots_stride;
+} omni_norm_rotary_args;
+int omni_norm_rotary(const omni_norm_rotary_args* args, omni_stream_t stream);
+
+/*
+ * omni_read_cache: the rows of slots (int32 / int64) as k and v [tokens][kv_heads][dim] of dtype (bf16,
+ * f16, f32), rounded once; a slot that is not in the cache gives zeros. dim a multiple of 16, rows of
+ * the cache 16-byte aligned; k and v of any alignment of their type. tokens = 0 does nothing.
+ */
+int omni_read_cache(const omni_kv_cache* cache, const void* slots, int slots_dtype,
+                    int64_t slots_stride, int64_t tokens, void* k, int64_t k_stride_token,
+                    int64_t k_stride_head, void* v, int64_t v_stride_token, int64_t v_stride_head,
+                    int dtype, omni_stream_t stream);
+
+/*
+ * omni_prompt_attention: attention of packed sequences. Sequence s has the queries starts[s] ..
+ * starts[s + 1] - 1 of q [tokens][heads][dim] and the keys key_starts[s] .. key_starts[s + 1] - 1 of k
+ * and v [key_tokens][kv_heads][dim] (bf16 or f16; starts int32 / int64, ascending, in device memory,
+ * clamped to [0, tokens] and [0, key_tokens]); query head h reads key head h / (heads / kv_heads).
+ * Causal: the last query sees all of its sequence's keys, each one before it one key less. A query that
+ * sees none, or whose scores are all -infinity, is zero; values behind what a query sees do not reach
+ * it, whatever they hold. Rows of out outside the sequences stay as they are; with clear_rest those
+ * from starts[sequences] on become zero. Scores, maxima and sums float32, softmax weights rounded to the
+ * type before they meet the values, outputs rounded once.
+ *
+ * Strides in elements, multiples of 8, at most 2^23 between tokens of k and v; pointers 16-byte aligned;
+ * dim a multiple of 8 up to 256; scale positive; out no input. tokens = 0 does nothing.
+ */
+typedef struct omni_prompt_args {
+  const void* q;
+  int64_t q_stride_token, q_stride_head;
+  const void* k;
+  int64_t k_stride_token, k_stride_head;
+  const void* v;
+  int64_t v_stride_token, v_stride_head;
+  void* out;
+  int64_t out_stride_token, out_stride_head;
+  int dtype;
+  int64_t tokens, key_tokens, heads, kv_heads, dim;
+  const void* starts;
+  const void* key_starts;
+  int starts_dtype;
+  int64_t sequences;
+  int causal;
+  float scale;
+  int clear_rest;
+} omni_prompt_args;
+int omni_prompt_attention(const omni_prompt_args* args, omni_stream_t stream);
+
+/*
+ * omni_paged_attention: one query of each sequence, q and out [batch][heads][dim] (bf16 or f16), over
+ * the first lengths[b] (int32 / int64) keys of its cache: key j lies on page table[b][j / page_size]
+ * (int32, rows table_stride apart), place j % page_size. The cache holds q's type or E4M3. Lengths count
+ * up to the table's table_columns pages and to max_length; a negative one is 0, and a sequence without
+ * keys is zero. Keys on pages outside [0, pages) are left out. Everything float32 but the products'
+ * operands; outputs rounded once. A row's bits depend on its own sequence alone.
+ *
+ * Strides of q and out in elements, multiples of 8, pointers and the cache's rows 16-byte aligned; dim a
+ * multiple of 16 up to 256; batch up to 65535; scale positive. workspace: with c = ceil(max_length /
+ * OMNI_PAGED_LEAST_CHUNK), and from 32 on max(32, ceil(max_length / OMNI_PAGED_MOST_CHUNK)), at least
+ * batch * heads * c * (dim + 2) * 4 bytes, 16-byte aligned; none for c up to 1. batch = 0 does nothing.
+ */
+enum { OMNI_PAGED_LEAST_CHUNK = 256, OMNI_PAGED_MOST_CHUNK = 1024 };
+typedef struct omni_paged_args {
+  const void* q;
+  int64_t q_stride_row, q_stride_head;
+  void* out;
+  int64_t out_stride_row, out_stride_head;
+  int dtype;
+  int64_t batch, heads;
+  const omni_kv_cache* cache;
+  const int32_t* table;
+  int64_t table_stride, table_columns;
+  const void* lengths;
+  int lengths_dtype;
+  int64_t max_length;
+  float scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} omni_paged_args;
+int omni_paged_attention(const omni_paged_args* args, omni_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,7 +33,7 @@ SOURCES = ["capi.hip", "rvq.hip", "conv.hip", "conv_k7_raw_wbf16.hip", "conv_k7_
            "egress.hip", "code2wav_front.hip", "channel_embedding.hip", "conv_general.hip",
            "conv_general_f32.hip", "conv_general_bf16.hip", "conv_general_f16.hip",
            "gemm.hip", "resblock_pair.hip", "block_fp8.hip", "gated_norm.hip", "rotary.hip",
-           "logits.hip"]
+           "logits.hip", "norm_rotary.hip", "prompt_attention.hip", "paged_attention.hip"]
 
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -1,0 +1,423 @@
+// Attention of one new token of each sequence over its paged key-value cache:
+//
+//   o = sum_j p_j v_j,   p_j = exp(scale q . k_j) / sum_j exp(scale q . k_j),   j < length
+//
+// for every head, the heads of a group over one key head. Rows of E4M3 count scale_j times their bytes.
+// A sequence without keys is zero. Keys on a page outside the cache are left out.
+//
+// The cache is read once, and that bounds it. A sequence's keys are cut into chunks whose size follows
+// from its length alone, so that a row's bits do not depend on the batch; a workgroup takes a chunk of a
+// key head for up to 16 query heads, its four waves every fourth tile of 32 keys each, with their own
+// running maximum and sum, joined through shared memory. One chunk is the result; several are joined by
+// a second launch, in their order.
+//
+// Scores transposed, S^T = K Q^T (16 x 16 x 32 MFMAs, K's rows from memory straight into operands: the
+// dimensions of a row in any order, so long as q's are in the same), and O^T = V^T P^T as in the prompt
+// kernel, V read transposed from shared memory. bf16 weights are held as a sum of two bf16 numbers, 16
+// bits of each weight: the matrix cores have nothing else to do here. 8-bit rows widen exactly; the keys'
+// scales multiply the scores and the values' the weights.
+#include <type_traits>
+
+#include "attention.h"
+
+namespace {
+
+struct PagedParams {
+  const uint8_t* q;
+  uint8_t* out;
+  int64_t q_row, q_head, out_row, out_head;  // bytes
+  CacheView cache;
+  const int32_t* table;
+  int64_t table_row;
+  const void* lengths;
+  int wide;
+  int64_t columns;  // of the table
+  int batch, kv_heads, group, head_tiles, dim;
+  float scale;  // of the scores, times log2(e)
+  float* parts;  // [batch][heads][chunks][dim], then [batch][heads][chunks][2] of maximum and sum
+  int chunks;    // most that a sequence has
+  int64_t max_length;
+};
+
+constexpr int kKeys = 32;  // of a tile
+constexpr int kWaves = 4;
+constexpr int kLeastChunk = OMNI_PAGED_LEAST_CHUNK, kMostChunk = OMNI_PAGED_MOST_CHUNK;
+
+// The keys of a chunk: the least of 256, 512 and 1024 that leaves a sequence at most 32 chunks, or 1024.
+// Short chunks spread one stream over the chip; long ones write fewer parts.
+OMNI_DEVICE int chunk_of(int64_t length) {
+  return length <= 32 * kLeastChunk ? kLeastChunk : length <= 64 * kLeastChunk ? 2 * kLeastChunk : kMostChunk;
+}
+
+// Eight E4M3 bytes as bf16 or float16, exactly.
+template <typename T>
+OMNI_DEVICE typename Op<T>::x8 widen(uint32_t lo, uint32_t hi);
+template <>
+OMNI_DEVICE bf16x8 widen<__bf16>(uint32_t lo, uint32_t hi) {
+  return widen8((int)lo, (int)hi);
+}
+template <>
+OMNI_DEVICE f16x8 widen<_Float16>(uint32_t lo, uint32_t hi) {
+  const i32x4 w = {
+      __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.f, false)),
+      __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.f, true)),
+      __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.f, false)),
+      __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.f, true))};
+  return __builtin_bit_cast(f16x8, w);
+}
+
+// The largest (the sum) over the four lanes that hold a query's scores: lanes 16 and 32 apart.
+OMNI_DEVICE float column_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+OMNI_DEVICE float column_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// V's LDS slot, of 16 bytes, of piece p of row r: read transposed, 4 rows 2 pieces of each at a time.
+template <int D>
+OMNI_DEVICE int v_slot(int r, int p) {
+  return D == 64 ? p ^ (((r >> 1) & 3) * 2) : p ^ ((r & 7) * 2);
+}
+
+// T: the type of q and out, H: of the cache's rows (uint8_t: E4M3). 16-bit rows are T. Weights go into the
+// product as PT: bf16 where the values' scales multiply them, whose range float16 has not.
+template <typename T, typename H, int D>
+__global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(const PagedParams p) {
+  constexpr bool kBytes = std::is_same<H, uint8_t>::value;
+  using PT = typename std::conditional<kBytes, __bf16, T>::type;
+  using O = Op<T>;
+  using P = Op<PT>;
+  constexpr bool kTwo = std::is_same<PT, __bf16>::value;
+  constexpr int kPieces = D / 8;  // 16-byte pieces of a row of values in shared memory
+  constexpr int kRow = D * (int)sizeof(H);
+  constexpr int kLoads = kRow / 64;        // 16-byte loads a lane and 16 keys: 4 lanes to a row
+  constexpr int kVLoads = kKeys * kRow / 1024;
+  // keys' rows (element offsets, negative: left out), their scales, V tiles of the waves; at the end
+  // the waves' outputs
+  __shared__ int64_t rows[kMostChunk];
+  __shared__ float scales[kBytes ? 2 : 1][kBytes ? kMostChunk : 1];
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[kWaves][kKeys * D * 2];
+  __shared__ float stats[kWaves][2][16];
+
+  const int lane = threadIdx.x & 63, column = lane & 15, quarter = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int chunk = blockIdx.x;
+  const int kv_head = blockIdx.y / p.head_tiles, head_tile = blockIdx.y % p.head_tiles;
+  const int b = blockIdx.z;
+  const int64_t given = p.wide ? static_cast<const int64_t*>(p.lengths)[b]
+                               : (int64_t) static_cast<const int32_t*>(p.lengths)[b];
+  const int64_t room = p.columns * p.cache.page_size;
+  const int64_t most = room < p.max_length ? room : p.max_length;
+  const int length = (int)(given < 0 ? 0 : given > most ? most : given);
+  const int size = chunk_of(length);
+  const int chunks = (length + size - 1) / size;
+  if (chunk > 0 && chunk >= chunks) return;
+  const int first = chunk * size, count = length - first < size ? length - first : size;
+
+  for (int i = threadIdx.x; i < count; i += 64 * kWaves) {
+    const uint32_t key = (uint32_t)(first + i), column_of = key / (uint32_t)p.cache.page_size;
+    const int page = p.table[b * p.table_row + column_of];
+    const uint32_t offset = key - column_of * (uint32_t)p.cache.page_size;
+    const bool held = page >= 0 && page < p.cache.pages;
+    rows[i] = held ? page * p.cache.page + offset * p.cache.token + kv_head * p.cache.head : -1;
+    if constexpr (kBytes) {
+      const int64_t at = (int64_t)page * p.cache.scale_page + offset * p.cache.scale_token +
+                         kv_head * p.cache.scale_head;
+      scales[0][i] = held ? p.cache.key_scale[at] : 0.f;
+      scales[1][i] = held ? p.cache.value_scale[at] : 0.f;
+    }
+  }
+
+  // q's operand: lane (column, quarter) holds of head `column` the dimensions that the same lane of a
+  // load holds of a key
+  const int head_in_group = head_tile * 16 + column;
+  const int head = kv_head * p.group + (head_in_group < p.group ? head_in_group : p.group - 1);
+  typename O::x8 q[D / 32];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    // of 16-bit rows load s holds dimensions 32 s + 8 quarter ..; of bytes load s / 2 64 (s / 2) + 16
+    // quarter .., its second half for odd s
+    const int d = kBytes ? (s / 2) * 64 + quarter * 16 + (s % 2) * 8 : s * 32 + quarter * 8;
+    if (d < p.dim)
+      q[s] = *reinterpret_cast<const typename O::x8*>(p.q + b * p.q_row + head * p.q_head + d * 2);
+    else
+      q[s] = typename O::x8{};
+  }
+
+  f32x4 o[D / 16];
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), l = 0.f;
+  __syncthreads();
+
+  const u32x4 nothing = {0u, 0u, 0u, 0u};
+  for (int at = wave * kKeys; at < count; at += kWaves * kKeys) {
+    u32x4 k[2][kLoads], v[kVLoads];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int i = at + t * 16 + column;
+      const int64_t row = i < count ? rows[i] : -1;
+#pragma unroll
+      for (int s = 0; s < kLoads; ++s) {
+        const int byte = s * 64 + quarter * 16;
+        k[t][s] = nothing;
+        if (row >= 0 && byte < p.dim * (int)sizeof(H))
+          k[t][s] = *reinterpret_cast<const u32x4*>(p.cache.keys + row * sizeof(H) + byte);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kVLoads; ++s) {
+      const int piece = s * 64 + lane, r = piece / (kRow / 16), byte = piece % (kRow / 16) * 16;
+      const int64_t row = at + r < count ? rows[at + r] : -1;
+      v[s] = nothing;
+      if (row >= 0 && byte < p.dim * (int)sizeof(H))
+        v[s] = *reinterpret_cast<const u32x4*>(p.cache.values + row * sizeof(H) + byte);
+    }
+
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        typename O::x8 a;
+        if constexpr (kBytes)
+          a = widen<T>(k[t][c / 2][c % 2 * 2], k[t][c / 2][c % 2 * 2 + 1]);
+        else
+          a = __builtin_bit_cast(typename O::x8, k[t][c]);
+        s[t] = O::mfma16(a, q[c], s[t]);
+      }
+    }
+    // V to shared memory as it will be read
+    uint8_t* tile = tiles[wave];
+#pragma unroll
+    for (int i = 0; i < kVLoads; ++i) {
+      const int piece = i * 64 + lane, r = piece / (kRow / 16), at16 = piece % (kRow / 16);
+      if constexpr (kBytes) {
+        const typename P::x8 x = widen<PT>(v[i][0], v[i][1]), y = widen<PT>(v[i][2], v[i][3]);
+        *reinterpret_cast<typename P::x8*>(tile + (r * kPieces + v_slot<D>(r, at16 * 2)) * 16) = x;
+        *reinterpret_cast<typename P::x8*>(tile + (r * kPieces + v_slot<D>(r, at16 * 2 + 1)) * 16) = y;
+      } else {
+        *reinterpret_cast<u32x4*>(tile + (r * kPieces + v_slot<D>(r, at16)) * 16) = v[i];
+      }
+    }
+
+    // lane (column, quarter) holds keys 16 t + 4 quarter .. + 3 of head `column`
+    float weight_scale[2][4];
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = at + t * 16 + quarter * 4 + e;
+        const bool seen = i < count && rows[i] >= 0;
+        if constexpr (kBytes) {
+          s[t][e] *= seen ? scales[0][i] : 0.f;
+          weight_scale[t][e] = seen ? scales[1][i] : 0.f;
+        }
+        s[t][e] = seen ? s[t][e] * p.scale : -__builtin_inff();
+        top = fmaxf(top, s[t][e]);
+      }
+    const float m_new = fmaxf(m, column_max(top));
+    const float m_use = m_new == -__builtin_inff() ? 0.f : m_new;
+    const float keep = __builtin_amdgcn_exp2f(m - m_use);
+    m = m_new;
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[d] *= keep;
+    typename P::x8 w, w_low;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = __builtin_amdgcn_exp2f(s[t][e] - m_use + P::kBias);
+        l += x;
+        if constexpr (kBytes) x *= weight_scale[t][e];
+        w[t * 4 + e] = (PT)x;
+        w_low[t * 4 + e] = (PT)(x - (float)w[t * 4 + e]);
+      }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const int r = quarter * 4 + (column >> 2), piece = d * 2 + ((column & 3) >> 1);
+      const int within = (column & 1) * 8;
+      const typename P::x8 a = __builtin_bit_cast(
+          typename P::x8,
+          read_transposed((const uint8_t OMNI_LDS*)(tile + (r * kPieces + v_slot<D>(r, piece)) * 16 + within),
+                          (const uint8_t OMNI_LDS*)(tile + ((r + 16) * kPieces + v_slot<D>(r + 16, piece)) * 16 +
+                                                    within)));
+      o[d] = P::mfma16(a, w, o[d]);
+      if constexpr (kTwo) o[d] = P::mfma16(a, w_low, o[d]);
+    }
+  }
+
+  // the waves' parts joined, in their order
+  l = column_sum(l);
+  if (quarter == 0) {
+    stats[wave][0][column] = m;
+    stats[wave][1][column] = l;
+  }
+  __syncthreads();  // and every wave has read its last tile
+  float m_all = stats[0][0][column];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, stats[w][0][column]);
+  const float m_use = m_all == -__builtin_inff() ? 0.f : m_all;
+  float l_all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    l_all += stats[w][1][column] * __builtin_amdgcn_exp2f(stats[w][0][column] - m_use);
+  const float keep = __builtin_amdgcn_exp2f(m - m_use);
+  // [16 heads][D + 4] of a wave at a time
+  constexpr int kPitch = D + 4;
+  static_assert(sizeof(tiles) >= 16 * kPitch * 4, "a wave's outputs fit the tiles");
+  float* sum = reinterpret_cast<float*>(tiles);
+  for (int turn = 0; turn < kWaves; ++turn) {
+    if (wave == turn) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        float* to = sum + column * kPitch + d * 16 + quarter * 4;
+        f32x4 x = o[d] * keep;
+        if (turn > 0) x += *reinterpret_cast<f32x4*>(to);
+        *reinterpret_cast<f32x4*>(to) = x;
+      }
+    }
+    __syncthreads();
+  }
+  // 16 heads' rows out: 16 threads to a head
+  const int h = threadIdx.x >> 4, part = threadIdx.x & 15;
+  const int out_in_group = head_tile * 16 + h;
+  if (out_in_group >= p.group) return;
+  const int out_head = kv_head * p.group + out_in_group;
+  // the statistics of head h: lane h's (any quarter's) of this wave
+  const float m_h = __shfl(m_all, h), l_h = __shfl(l_all, h);
+  if (chunks > 1) {
+    const int64_t at = ((int64_t)b * p.kv_heads * p.group + out_head) * p.chunks + chunk;
+    for (int d = part * 4; d < p.dim; d += 64)
+      *reinterpret_cast<f32x4*>(p.parts + at * p.dim + d) = *reinterpret_cast<f32x4*>(sum + h * kPitch + d);
+    if (part == 0) {
+      float* to = p.parts + (int64_t)p.batch * p.kv_heads * p.group * p.chunks * p.dim + at * 2;
+      to[0] = m_h;
+      to[1] = l_h;
+    }
+    return;
+  }
+  const float unit = m_h == -__builtin_inff() ? 0.f : 1.f / l_h;
+  T* to = reinterpret_cast<T*>(p.out + b * p.out_row + out_head * p.out_head);
+  for (int d = part * 4; d < p.dim; d += 64) {
+    const f32x4 x = *reinterpret_cast<f32x4*>(sum + h * kPitch + d);
+    typename O::x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * unit);
+    *reinterpret_cast<typename O::x4*>(to + d) = y;
+  }
+}
+
+// The chunks of a (sequence, head) joined in their order: a workgroup, a thread to a dimension.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
+  const int heads = p.kv_heads * p.group;
+  const int b = blockIdx.x / heads, head = blockIdx.x % heads;
+  const int64_t given = p.wide ? static_cast<const int64_t*>(p.lengths)[b]
+                               : (int64_t) static_cast<const int32_t*>(p.lengths)[b];
+  const int64_t room = p.columns * p.cache.page_size;
+  const int64_t most = room < p.max_length ? room : p.max_length;
+  const int length = (int)(given < 0 ? 0 : given > most ? most : given);
+  const int size = chunk_of(length), chunks = (length + size - 1) / size;
+  if (chunks <= 1) return;
+  const int64_t at = ((int64_t)b * heads + head) * p.chunks;
+  const float* stats = p.parts + (int64_t)p.batch * heads * p.chunks * p.dim + at * 2;
+  float m = -__builtin_inff();
+  for (int c = 0; c < chunks; ++c) m = fmaxf(m, stats[2 * c]);
+  const float m_use = m == -__builtin_inff() ? 0.f : m;
+  for (int d = threadIdx.x; d < p.dim; d += blockDim.x) {
+    float l = 0.f, o = 0.f;
+    for (int c = 0; c < chunks; ++c) {
+      const float keep = __builtin_amdgcn_exp2f(stats[2 * c] - m_use);
+      l = __builtin_fmaf(stats[2 * c + 1], keep, l);
+      o = __builtin_fmaf(p.parts[(at + c) * p.dim + d], keep, o);
+    }
+    reinterpret_cast<T*>(p.out + b * p.out_row + head * p.out_head)[d] =
+        (T)(m == -__builtin_inff() ? 0.f : o / l);
+  }
+}
+
+template <typename T, typename H, int D>
+int launch_paged(const PagedParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_kernel<T, H, D>),
+                     dim3((unsigned)p.chunks, (unsigned)(p.kv_heads * p.head_tiles), (unsigned)p.batch),
+                     dim3(64 * kWaves), 0, stream, p);
+  OMNI_LAUNCH_CHECK();
+  if (p.chunks > 1) {
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(p.batch * p.kv_heads * p.group)), dim3(D < 128 ? 64 : 128),
+                       0, stream, p);
+    OMNI_LAUNCH_CHECK();
+  }
+  return OMNI_OK;
+}
+
+template <typename T, typename H>
+int launch_dim(const PagedParams& p, hipStream_t stream) {
+  if (p.dim <= 64) return launch_paged<T, H, 64>(p, stream);
+  if (p.dim <= 128) return launch_paged<T, H, 128>(p, stream);
+  return launch_paged<T, H, 256>(p, stream);
+}
+
+}  // namespace
+
+extern "C" int omni_paged_attention(const omni_paged_args* a, omni_stream_t stream) {
+  if (!a || !a->cache || a->batch < 0 || a->heads < 1 || a->cache->kv_heads < 1 ||
+      a->heads % a->cache->kv_heads || a->heads > 65535 || a->cache->dim < 16 || a->cache->dim % 16 ||
+      a->table_columns < 0 || a->max_length < 0 || !(a->scale > 0.f) || !(a->scale <= 3.0e38f) ||
+      (a->dtype != OMNI_DTYPE_BF16 && a->dtype != OMNI_DTYPE_F16) ||
+      (a->cache->dtype != OMNI_DTYPE_FP8_E4M3 && a->cache->dtype != a->dtype) ||
+      (a->lengths_dtype != OMNI_DTYPE_I32 && a->lengths_dtype != OMNI_DTYPE_I64))
+    return OMNI_ERR_INVALID_ARG;
+  const int64_t strides[] = {a->q_stride_row, a->q_stride_head, a->out_stride_row, a->out_stride_head};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return OMNI_ERR_INVALID_ARG;
+  PagedParams p{};
+  if (!cache_view(*a->cache, 16, &p.cache)) return OMNI_ERR_INVALID_ARG;
+  if (a->cache->dim > 256 || a->batch > 65535 || a->max_length > 0x7ffffc00LL) return OMNI_ERR_UNSUPPORTED;
+  if (a->batch == 0) return OMNI_OK;
+  if (!a->q || !a->out || !a->lengths || (a->table_columns > 0 && !a->table) || !aligned_to(a->q, 16) ||
+      !aligned_to(a->out, 16) || !aligned_to(a->table, 4) ||
+      !aligned_to(a->lengths, a->lengths_dtype == OMNI_DTYPE_I64 ? 8 : 4))
+    return OMNI_ERR_INVALID_ARG;
+  const int64_t kv_heads = a->cache->kv_heads, group = a->heads / kv_heads;
+  const int64_t tiles = (group + 15) / 16;
+  if (kv_heads * tiles > 65535 || a->batch * a->heads > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+  // the most chunks of a length up to max_length: 32 up to 16384 keys, then one for each 1024
+  const int64_t few = (a->max_length + kLeastChunk - 1) / kLeastChunk;
+  const int64_t many = (a->max_length + kMostChunk - 1) / kMostChunk;
+  const int64_t chunks = few < 32 ? (few > 0 ? few : 1) : many > 32 ? many : 32;
+  if (chunks > 1 && (!a->workspace || !aligned_to(a->workspace, 16) ||
+                     a->workspace_bytes < a->batch * a->heads * chunks * (a->cache->dim + 2) * 4))
+    return OMNI_ERR_INVALID_ARG;
+  p.q = static_cast<const uint8_t*>(a->q);
+  p.out = static_cast<uint8_t*>(a->out);
+  p.q_row = a->q_stride_row * 2;
+  p.q_head = a->q_stride_head * 2;
+  p.out_row = a->out_stride_row * 2;
+  p.out_head = a->out_stride_head * 2;
+  p.table = static_cast<const int32_t*>(a->table);
+  p.table_row = a->table_stride;
+  p.lengths = a->lengths;
+  p.wide = a->lengths_dtype == OMNI_DTYPE_I64;
+  p.columns = a->table_columns;
+  p.batch = (int)a->batch;
+  p.kv_heads = (int)kv_heads;
+  p.group = (int)group;
+  p.head_tiles = (int)tiles;
+  p.dim = (int)a->cache->dim;
+  p.scale = a->scale * kLog2e;
+  p.parts = static_cast<float*>(a->workspace);
+  p.chunks = (int)chunks;
+  p.max_length = a->max_length;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool bytes = a->cache->dtype == OMNI_DTYPE_FP8_E4M3;
+  if (a->dtype == OMNI_DTYPE_BF16)
+    return bytes ? launch_dim<__bf16, uint8_t>(p, s) : launch_dim<__bf16, __bf16>(p, s);
+  return bytes ? launch_dim<_Float16, uint8_t>(p, s) : launch_dim<_Float16, _Float16>(p, s);
+}

@@ -1,0 +1,368 @@
+// Attention of whole prompts: packed sequences, each with its own number of queries and keys, heads
+// grouped over key heads,
+//
+//   o_i = sum_j p_ij v_j,   p_ij = exp(scale q_i . k_j) / sum_j exp(scale q_i . k_j)
+//
+// over the keys j that query i sees: all of its sequence, or with `causal` those up to its own place
+// when the last query stands at the last key. A query that sees none is zero.
+//
+// One pass over the keys with the running maximum m and sum l of a softmax. A wave owns 32 rows; a row
+// is a (query, head) pair, the heads of a group side by side, so that a tile of keys in shared memory
+// serves the whole group. Scores are computed transposed, S^T = K Q^T (32 x 32 x 16 MFMAs, a lane's
+// column one row's scores), so that a row's maximum is a lane's own but for one swap of half-waves, and
+// P^T is the B operand of O^T = V^T P^T as it stands: of each 16 keys, lanes below 32 hold 0 .. 3 and 8
+// .. 11, the others 4 .. 7 and 12 .. 15, and V^T, read transposed, takes its keys in that order. The
+// weights are rounded to the rows' type for that product (half a step of each, the sum l is of the
+// unrounded ones); scores, maxima, sums and outputs are float32.
+#include "attention.h"
+
+namespace {
+
+struct PromptParams {
+  const uint8_t* q;
+  const uint8_t* k;
+  const uint8_t* v;
+  uint8_t* out;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;  // bytes
+  const void* starts;
+  const void* key_starts;
+  int wide;  // the starts are int64
+  int64_t tokens, key_tokens;
+  int sequences;  // and one past them where the rows behind the last one are cleared
+  int cleared;
+  int kv_heads, group, dim, causal;
+  float scale;  // of the scores, times log2(e)
+  int slots;    // row tiles a key head, an upper bound
+};
+
+constexpr int kKeys = 64;  // of a tile
+
+OMNI_DEVICE int64_t start_of(const void* starts, int wide, int64_t at, int64_t end) {
+  const int64_t s = wide ? static_cast<const int64_t*>(starts)[at]
+                         : (int64_t) static_cast<const int32_t*>(starts)[at];
+  return s < 0 ? 0 : s > end ? end : s;
+}
+
+// The LDS slot, of 16 bytes, that piece p of key row r takes in its row: K's rows are read 16 bytes a
+// lane, 32 consecutive rows the same piece; V's transposed, 8 consecutive rows 4 pieces of each.
+template <int D>
+OMNI_DEVICE int k_slot(int r, int p) {
+  return D == 64 ? p ^ ((r >> 1) & 7) : p ^ (r & 15);
+}
+template <int D>
+OMNI_DEVICE int v_slot(int r, int p) {
+  return D == 64 ? p ^ (((r >> 1) & 1) * 4) : p ^ ((r & 3) * 4);
+}
+
+template <typename T, int D, int NW>
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const PromptParams p) {
+  using O = Op<T>;
+  constexpr int kRows = 32 * NW;
+  constexpr int kPieces = D / 8;  // 16-byte pieces of a row
+  constexpr int kTile = kKeys * D * 2;
+  constexpr int kDma = kKeys * kPieces / 64 / NW;  // instructions a wave and tile
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2][K, V]
+  const int lane = threadIdx.x & 63, half = lane >> 5, column = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+
+  // Key head fastest: the 8 XCDs take workgroups in turn, so with 8 (4, 2) key heads each XCD's L2
+  // holds its own head's keys. The last tiles of a sequence, which see the most keys, go first.
+  const int kv_head = blockIdx.x % p.kv_heads;
+  const int slot = p.slots - 1 - blockIdx.x / p.kv_heads;
+  // Sequence s owns the tiles from floor(first row / kRows) + s on: never fewer than it needs, and
+  // found by search without a sum over the sequences before it.
+  int lo = 0, n = p.sequences;
+  while (n > 1) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const bool before =
+        at < n && start_of(p.starts, p.wide, lo + at, p.tokens) * p.group / kRows + lo + at <= slot;
+    const int found = __builtin_popcountll(__ballot(before));
+    const int skip = found > 0 ? (found - 1) * step : 0;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  const int seq = __builtin_amdgcn_readfirstlane(lo);
+  const int64_t first = start_of(p.starts, p.wide, seq, p.tokens);
+  const bool rest = p.cleared && seq == p.sequences - 1;  // the rows behind the last sequence
+  const int64_t last = rest ? p.tokens : start_of(p.starts, p.wide, seq + 1, p.tokens);
+  const int64_t queries = last - first;
+  const int64_t row0 = (slot - (first * p.group / kRows + seq)) * kRows;
+  if (queries <= 0 || row0 < 0 || row0 >= queries * p.group) return;
+  const int64_t key_first = rest ? 0 : start_of(p.key_starts, p.wide, seq, p.key_tokens);
+  int64_t keys = rest ? 0 : start_of(p.key_starts, p.wide, seq + 1, p.key_tokens) - key_first;
+  if (keys < 0) keys = 0;
+
+  // this lane's row, and how many keys it, the wave's first and last row and the tile's last see
+  const int64_t wave_row = row0 + wave * 32, rows = queries * p.group;
+  const int64_t row = wave_row + column < rows ? wave_row + column : rows - 1;
+  const int64_t query = row / p.group;
+  const int head = kv_head * p.group + (int)(row - query * p.group);
+  const int64_t ahead = p.causal ? keys - queries + 1 : keys;
+  auto seen_by = [&](int64_t r) {
+    const int64_t s = p.causal ? (r < rows ? r : rows - 1) / p.group + ahead : ahead;
+    return (int)(s < 0 ? 0 : s);
+  };
+  const int seen = seen_by(row);
+  const int seen_least = __builtin_amdgcn_readfirstlane(seen_by(wave_row));
+  const int seen_most = wave_row < rows ? __builtin_amdgcn_readfirstlane(seen_by(wave_row + 31)) : 0;
+  const int tiles = (__builtin_amdgcn_readfirstlane(seen_by(row0 + kRows - 1)) + kKeys - 1) / kKeys;
+
+  typename O::x8 q[D / 16];
+  {
+    const uint8_t* from = p.q + (first + query) * p.q_token + head * p.q_head + half * 16;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      if (s * 16 + half * 8 < p.dim)
+        q[s] = *reinterpret_cast<const typename O::x8*>(from + s * 32);
+      else
+        q[s] = typename O::x8{};
+    }
+  }
+
+  // DMA: instruction i of the wave fills slots 64 (wave kDma + i) .. of the tile; the row and piece
+  // that belong there
+  uint32_t k_off[kDma], v_off[kDma];
+#pragma unroll
+  for (int i = 0; i < kDma; ++i) {
+    const int at = (wave * kDma + i) * 64 + lane, r = at / kPieces, s = at % kPieces;
+    const int kp = k_slot<D>(r, s), vp = v_slot<D>(r, s);
+    k_off[i] = kp * 8 < p.dim ? (uint32_t)(r * p.k_token + kp * 16) : kOutOfRange;
+    v_off[i] = vp * 8 < p.dim ? (uint32_t)(r * p.v_token + vp * 16) : kOutOfRange;
+  }
+  const uint8_t* k_base = p.k + key_first * p.k_token + kv_head * p.k_head;
+  const uint8_t* v_base = p.v + key_first * p.v_token + kv_head * p.v_head;
+  // rows behind the sequence's last key are zeros
+  auto issue = [&](int tile) __attribute__((always_inline)) {
+    const int64_t at = (int64_t)tile * kKeys;
+    const int valid = (int)(keys - at < kKeys ? keys - at : kKeys);
+    const auto kr = buffer_rsrc(k_base + at * p.k_token, (uint32_t)((valid - 1) * p.k_token + p.dim * 2));
+    const auto vr = buffer_rsrc(v_base + at * p.v_token, (uint32_t)((valid - 1) * p.v_token + p.dim * 2));
+    uint8_t* stage = lds + (tile & 1) * 2 * kTile + wave * kDma * 1024;
+#pragma unroll
+    for (int i = 0; i < kDma; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (OMNI_LDS void*)(stage + i * 1024), 16, (int)k_off[i],
+                                               0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kDma; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (OMNI_LDS void*)(stage + kTile + i * 1024), 16,
+                                               (int)v_off[i], 0, 0, 0);
+  };
+
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;
+
+  // V's operand of 16 keys (from c on) and 32 dimensions (block d): two transposed reads
+  auto v_operand = [&](const uint8_t* vt, int c, int d) __attribute__((always_inline)) {
+    const int r = c + half * 4 + ((lane & 15) >> 2), r2 = r + 8;
+    const int piece = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), within = (lane & 1) * 8;
+    const s16x8 x = read_transposed(
+        (const uint8_t OMNI_LDS*)(vt + (r * kPieces + v_slot<D>(r, piece)) * 16 + within),
+        (const uint8_t OMNI_LDS*)(vt + (r2 * kPieces + v_slot<D>(r2, piece)) * 16 + within));
+    return __builtin_bit_cast(typename O::x8, x);
+  };
+
+  if (tiles > 0) issue(tiles - 1);
+  for (int tile = tiles - 1; tile >= 0; --tile) {
+    // the tile has arrived in every wave, and every wave has read the one before, whose place the next
+    // one takes
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    if (tile > 0) issue(tile - 1);
+    const int first_key = tile * kKeys;
+    if (first_key >= seen_most) continue;
+    const bool partial = first_key + kKeys > seen_least;
+    const uint8_t* kt = lds + (tile & 1) * 2 * kTile;
+    const uint8_t* vt = kt + kTile;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+      const int r = b * 32 + column;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        const typename O::x8 a = *reinterpret_cast<const typename O::x8*>(
+            kt + (r * kPieces + k_slot<D>(r, c * 2 + half)) * 16);
+        s[b] = O::mfma32(a, q[c], s[b]);
+      }
+    }
+    if (partial) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = first_key + b * 32 + (i / 4) * 8 + half * 4 + i % 4;
+          s[b][i] = key < seen ? s[b][i] : -__builtin_inff();
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = half_max(top) * p.scale;
+    const float m_new = fmaxf(m, top);
+    // a row that has seen nothing yet: its weights are exp2(-infinity - 0)
+    const float m_use = m_new == -__builtin_inff() ? 0.f : m_new;
+    const float keep = __builtin_amdgcn_exp2f(m - m_use);
+    m = m_new;
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+    typename O::x8 w[4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], p.scale, O::kBias - m_use));
+        l += x;
+        w[b * 2 + i / 8][i % 8] = (T)x;
+      }
+
+    bool poisoned = false;
+    if (partial) {
+      // A key that some of these rows do not see may hold an infinity or a NaN, and zero times it is
+      // one too: such a tile's sum over zeros is not zero.
+      f32x16 zeros;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) zeros[i] = 0.f;
+      const typename O::x8 none{};
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) zeros = O::mfma32(v_operand(vt, c * 16, d), none, zeros);
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bad |= zeros[i] != 0.f;
+      poisoned = __ballot(bad) != 0;
+    }
+    if (!poisoned) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) o[d] = O::mfma32(v_operand(vt, c * 16, d), w[c], o[d]);
+    } else {
+      // each key's contribution on its own, added where it is seen
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+          const typename O::x8 v = v_operand(vt, c * 16, d);
+#pragma unroll 1
+          for (int e = 0; e < 16; ++e) {
+            const bool mine = half == e / 8;
+            typename O::x8 ve, we;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              ve[j] = mine && j == e % 8 ? v[j] : (T)0.f;
+              we[j] = mine && j == e % 8 ? w[c][j] : (T)0.f;
+            }
+            f32x16 part;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) part[i] = 0.f;
+            part = O::mfma32(ve, we, part);
+            const int key = first_key + c * 16 + (e % 8 / 4) * 8 + (e / 8) * 4 + e % 4;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] += key < seen ? part[i] : 0.f;
+          }
+        }
+    }
+  }
+
+  if (wave_row + column >= rows) return;
+  l = half_sum(l);
+  const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
+  uint8_t* to = p.out + (first + query) * p.out_token + head * p.out_head + half * 8;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (d * 32 + i * 8 + half * 4 >= p.dim) continue;
+      typename O::x4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = (T)(o[d][i * 4 + j] * unit);
+      *reinterpret_cast<typename O::x4*>(to + d * 64 + i * 16) = x;
+    }
+}
+
+template <typename T, int D, int NW>
+int launch_prompt(PromptParams p, hipStream_t stream) {
+  constexpr int kLds = 2 * 2 * kKeys * D * 2;
+  const int64_t slots = p.tokens * p.group / (32 * NW) + p.sequences;
+  if (slots * p.kv_heads > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+  p.slots = (int)slots;
+  if (kLds > 64 * 1024) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, D, NW>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
+      return OMNI_ERR_LAUNCH;
+  }
+  hipLaunchKernelGGL((prompt_kernel<T, D, NW>), dim3((unsigned)(slots * p.kv_heads)), dim3(64 * NW), kLds,
+                     stream, p);
+  OMNI_LAUNCH_CHECK();
+  return OMNI_OK;
+}
+
+template <typename T>
+int launch_dim(const PromptParams& p, hipStream_t stream) {
+  if (p.dim <= 64) return launch_prompt<T, 64, 4>(p, stream);
+  if (p.dim <= 128) return launch_prompt<T, 128, 4>(p, stream);
+  return launch_prompt<T, 256, 4>(p, stream);
+}
+
+}  // namespace
+
+extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t stream) {
+  if (!a || a->tokens < 0 || a->key_tokens < 0 || a->sequences < 0 || a->heads < 1 || a->kv_heads < 1 ||
+      a->heads % a->kv_heads || a->heads > 65536 || a->dim < 8 || a->dim % 8 || !(a->scale > 0.f) ||
+      !(a->scale <= 3.0e38f) || a->sequences > 0x7ffffff0LL ||
+      (a->dtype != OMNI_DTYPE_BF16 && a->dtype != OMNI_DTYPE_F16) ||
+      (a->starts_dtype != OMNI_DTYPE_I32 && a->starts_dtype != OMNI_DTYPE_I64))
+    return OMNI_ERR_INVALID_ARG;
+  if (a->dim > 256 || a->key_tokens > 0x7fffff00LL || a->tokens > 0x7fffff00LL) return OMNI_ERR_UNSUPPORTED;
+  const int64_t strides[] = {a->q_stride_token, a->q_stride_head, a->k_stride_token, a->k_stride_head,
+                             a->v_stride_token, a->v_stride_head, a->out_stride_token, a->out_stride_head};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return OMNI_ERR_INVALID_ARG;
+  // a tile's keys lie within a buffer's 2 GiB
+  if (a->k_stride_token > (1 << 23) || a->v_stride_token > (1 << 23)) return OMNI_ERR_UNSUPPORTED;
+  const int index = a->starts_dtype == OMNI_DTYPE_I64 ? 8 : 4;
+  if (a->tokens == 0 || (a->sequences == 0 && !a->clear_rest)) return OMNI_OK;
+  if (!a->q || !a->out || !a->starts || !a->key_starts || (a->key_tokens > 0 && (!a->k || !a->v)) ||
+      !aligned_to(a->q, 16) || !aligned_to(a->k, 16) || !aligned_to(a->v, 16) || !aligned_to(a->out, 16) ||
+      !aligned_to(a->starts, index) || !aligned_to(a->key_starts, index))
+    return OMNI_ERR_INVALID_ARG;
+  PromptParams p{};
+  p.q = static_cast<const uint8_t*>(a->q);
+  p.k = static_cast<const uint8_t*>(a->k);
+  p.v = static_cast<const uint8_t*>(a->v);
+  p.out = static_cast<uint8_t*>(a->out);
+  p.q_token = a->q_stride_token * 2;
+  p.q_head = a->q_stride_head * 2;
+  p.k_token = a->k_stride_token * 2;
+  p.k_head = a->k_stride_head * 2;
+  p.v_token = a->v_stride_token * 2;
+  p.v_head = a->v_stride_head * 2;
+  p.out_token = a->out_stride_token * 2;
+  p.out_head = a->out_stride_head * 2;
+  p.starts = a->starts;
+  p.key_starts = a->key_starts;
+  p.wide = a->starts_dtype == OMNI_DTYPE_I64;
+  p.tokens = a->tokens;
+  p.key_tokens = a->key_tokens;
+  p.cleared = a->clear_rest ? 1 : 0;
+  p.sequences = (int)a->sequences + p.cleared;
+  p.kv_heads = (int)a->kv_heads;
+  p.group = (int)(a->heads / a->kv_heads);
+  p.dim = (int)a->dim;
+  p.causal = a->causal ? 1 : 0;
+  p.scale = a->scale * kLog2e;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return a->dtype == OMNI_DTYPE_BF16 ? launch_dim<__bf16>(p, s) : launch_dim<_Float16>(p, s);
+}

@@ -326,6 +326,128 @@ class LogitsArgs(ctypes.Structure):
     ]
 
 
+class KvCacheStruct(ctypes.Structure):
+    """Mirror of ``omni_kv_cache`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("stride_page", ctypes.c_int64),
+        ("stride_head", ctypes.c_int64),
+        ("stride_token", ctypes.c_int64),
+        ("key_scale", ctypes.c_void_p),
+        ("value_scale", ctypes.c_void_p),
+        ("scale_stride_page", ctypes.c_int64),
+        ("scale_stride_head", ctypes.c_int64),
+        ("scale_stride_token", ctypes.c_int64),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+    ]
+
+
+class NormRotaryArgs(ctypes.Structure):
+    """Mirror of ``omni_norm_rotary_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v", ctypes.c_void_p),
+        ("v_stride_token", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_stride_token", ctypes.c_int64),
+        ("q_out_stride_head", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p),
+        ("k_out_stride_token", ctypes.c_int64),
+        ("k_out_stride_head", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+        ("normed", ctypes.c_int),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("pairs", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("positions_dtype", ctypes.c_int),
+        ("positions_stride", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p),
+        ("factor", ctypes.c_float),
+        ("layout", ctypes.c_int),
+        ("cache", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("slots_dtype", ctypes.c_int),
+        ("slots_stride", ctypes.c_int64),
+    ]
+
+
+class PromptArgs(ctypes.Structure):
+    """Mirror of ``omni_prompt_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v", ctypes.c_void_p),
+        ("v_stride_token", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride_token", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("tokens", ctypes.c_int64),
+        ("key_tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+        ("starts", ctypes.c_void_p),
+        ("key_starts", ctypes.c_void_p),
+        ("starts_dtype", ctypes.c_int),
+        ("sequences", ctypes.c_int64),
+        ("causal", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("clear_rest", ctypes.c_int),
+    ]
+
+
+class PagedArgs(ctypes.Structure):
+    """Mirror of ``omni_paged_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_row", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride_row", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("cache", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("table_columns", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("lengths_dtype", ctypes.c_int),
+        ("max_length", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 _FORMATS = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int: "i", ctypes.c_float: "f"}
 
 
@@ -340,7 +462,12 @@ pack_block_fp8 = _packer(BlockFp8Args)
 pack_gated_norm = _packer(GatedNormArgs)
 pack_rotary = _packer(RotaryArgs)
 pack_logits = _packer(LogitsArgs)
+pack_kv_cache = _packer(KvCacheStruct)
+pack_norm_rotary = _packer(NormRotaryArgs)
+pack_prompt = _packer(PromptArgs)
+pack_paged = _packer(PagedArgs)
 BLOCK_FP8_FEW_ROWS = 16
+PAGED_LEAST_CHUNK, PAGED_MOST_CHUNK = 256, 1024
 
 GEMM_STORE, GEMM_SILU_MUL, GEMM_GELU, GEMM_SCALED_RESIDUAL = 0, 1, 2, 3
 NORM_RMS, NORM_LAYER = 0, 1
@@ -416,6 +543,10 @@ SIGNATURES: dict[str, list] = {
     "omni_gated_residual_norm": [ctypes.c_char_p, _PTR],
     "omni_rotary": [ctypes.c_char_p, _PTR],
     "omni_adjust_logits": [ctypes.c_char_p, _PTR],
+    "omni_norm_rotary": [ctypes.c_char_p, _PTR],
+    "omni_read_cache": [_PTR, _PTR, _INT, _I64, _I64, _PTR, _I64, _I64, _PTR, _I64, _I64, _INT, _PTR],
+    "omni_prompt_attention": [ctypes.c_char_p, _PTR],
+    "omni_paged_attention": [ctypes.c_char_p, _PTR],
 }
 _RESTYPES = {"omni_codec_error_string": ctypes.c_char_p}
 
@@ -516,6 +647,18 @@ def stream_handle(device: torch.device | None = None) -> int:
             and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def launch_on(index: int, entry, *args) -> int:
+    """entry(*args, stream): the current stream of GPU `index`, which need not be the current GPU. A
+    default stream's handle says nothing of its GPU, so the call is made with that one current."""
+    if _current_device is None or _current_device() == index:
+        return entry(*args, raw_stream(index))
+    with torch.cuda.device(index):
+        return entry(*args, raw_stream(index))
 
 
 def row_stride(t: torch.Tensor) -> int:
