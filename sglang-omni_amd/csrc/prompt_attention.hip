@@ -36,6 +36,7 @@ struct PromptParams {
 };
 
 constexpr int kKeys = 64;  // of a tile
+constexpr float kLazy = 6.f;
 
 OMNI_DEVICE int64_t start_of(const void* starts, int wide, int64_t at, int64_t end) {
   const int64_t s = wide ? static_cast<const int64_t*>(starts)[at]
@@ -153,44 +154,96 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-  float m = -__builtin_inff(), l = 0.f;
+  float m = -__builtin_inff(), m_use = 0.f, l = 0.f;
 
-  // V's operand of 16 keys (from c on) and 32 dimensions (block d): two transposed reads
-  auto v_operand = [&](const uint8_t* vt, int c, int d) __attribute__((always_inline)) {
-    const int r = c + half * 4 + ((lane & 15) >> 2), r2 = r + 8;
-    const int piece = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), within = (lane & 1) * 8;
-    const s16x8 x = read_transposed(
-        (const uint8_t OMNI_LDS*)(vt + (r * kPieces + v_slot<D>(r, piece)) * 16 + within),
-        (const uint8_t OMNI_LDS*)(vt + (r2 * kPieces + v_slot<D>(r2, piece)) * 16 + within));
-    return __builtin_bit_cast(typename O::x8, x);
+  // Where this lane reads in a tile: K's row `column` for each step of 16 dimensions (the second 32 keys
+  // lie 32 rows on), V's for each block of 32 dimensions (16 keys 16 rows on, an operand's second four 8).
+  constexpr int kPitch = D * 2;
+  int k_at[D / 16], v_at[D / 32];
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) k_at[c] = column * kPitch + k_slot<D>(column, c * 2 + half) * 16;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) {
+    const int r = half * 4 + ((lane & 15) >> 2), piece = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    v_at[d] = kTile + r * kPitch + v_slot<D>(r, piece) * 16 + (lane & 1) * 8;
+  }
+  const uint8_t OMNI_LDS* shared = (const uint8_t OMNI_LDS*)lds;
+  auto k_operand = [&](int stage, int b, int c) __attribute__((always_inline)) {
+    return *(const typename O::x8 OMNI_LDS*)(shared + k_at[c] + (stage * 2 * kTile + b * 32 * kPitch));
   };
-
-  if (tiles > 0) issue(tiles - 1);
-  for (int tile = tiles - 1; tile >= 0; --tile) {
-    // the tile has arrived in every wave, and every wave has read the one before, whose place the next
-    // one takes
+  auto v_operand = [&](int stage, int c, int d) __attribute__((always_inline)) {
+    const uint8_t OMNI_LDS* at = shared + v_at[d] + (stage * 2 * kTile + c * 16 * kPitch);
+    return __builtin_bit_cast(typename O::x8, read_transposed(at, at + 8 * kPitch));
+  };
+  // the tile has arrived in every wave, and every wave has read the one before, whose place the next
+  // one takes
+  auto arrive = [&](int tile) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     asm volatile("s_barrier" ::: "memory");
     if (tile > 0) issue(tile - 1);
-    const int first_key = tile * kKeys;
-    if (first_key >= seen_most) continue;
-    const bool partial = first_key + kKeys > seen_least;
-    const uint8_t* kt = lds + (tile & 1) * 2 * kTile;
-    const uint8_t* vt = kt + kTile;
-
-    f32x16 s[2];
+  };
+  auto scores_of = [&](int stage, f32x16 (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-      const int r = b * 32 + column;
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        const typename O::x8 a = *reinterpret_cast<const typename O::x8*>(
-            kt + (r * kPieces + k_slot<D>(r, c * 2 + half)) * 16);
-        s[b] = O::mfma32(a, q[c], s[b]);
-      }
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] = O::mfma32(k_operand(stage, b, c), q[c], s[b]);
+  };
+  // The weights of a tile's scores. The maximum they are taken against moves only where a score is past
+  // it by more than 2^kLazy: until then weights are that much larger, which costs no precision, and the
+  // sums and outputs need no rescaling.
+  auto weights_of = [&](const f32x16 (&s)[2], typename O::x8 (&w)[4]) __attribute__((always_inline)) {
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = half_max(top) * p.scale;
+    if (__ballot(top > m + kLazy) != 0) {
+      const float m_new = fmaxf(m, top);
+      // a row that has seen nothing yet: its weights are exp2(-infinity - 0)
+      m_use = m_new == -__builtin_inff() ? 0.f : m_new;
+      const float keep = __builtin_amdgcn_exp2f(m - m_use);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= keep;
     }
+    const float shift = O::kBias - m_use;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], p.scale, shift));
+        l += x;
+        w[b * 2 + i / 8][i % 8] = (T)x;
+      }
+  };
+  auto accumulate = [&](int stage, const typename O::x8 (&w)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) o[d] = O::mfma32(v_operand(stage, c, d), w[c], o[d]);
+  };
+
+  if (tiles > 0) issue(tiles - 1);
+  // Tiles from the last: first those that some row of the workgroup does not see whole (and one more
+  // where the next would not be in the first stage).
+  int tile = tiles - 1;
+  const int whole = __builtin_amdgcn_readfirstlane(seen_by(row0)) / kKeys;  // tiles that every row sees
+  for (; tile >= 0 && (tile >= whole || tile % 2 == 1); --tile) {
+    arrive(tile);
+    const int first_key = tile * kKeys, stage = tile & 1;
+    if (first_key >= seen_most) continue;
+    f32x16 s[2];
+    scores_of(stage, s);
+    const bool partial = first_key + kKeys > seen_least;
+    bool poisoned = false;
     if (partial) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -200,33 +253,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
           s[b][i] = key < seen ? s[b][i] : -__builtin_inff();
         }
     }
-    float top = s[0][0];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    top = half_max(top) * p.scale;
-    const float m_new = fmaxf(m, top);
-    // a row that has seen nothing yet: its weights are exp2(-infinity - 0)
-    const float m_use = m_new == -__builtin_inff() ? 0.f : m_new;
-    const float keep = __builtin_amdgcn_exp2f(m - m_use);
-    m = m_new;
-    l *= keep;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] *= keep;
     typename O::x8 w[4];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], p.scale, O::kBias - m_use));
-        l += x;
-        w[b * 2 + i / 8][i % 8] = (T)x;
-      }
-
-    bool poisoned = false;
+    weights_of(s, w);
     if (partial) {
       // A key that some of these rows do not see may hold an infinity or a NaN, and zero times it is
       // one too: such a tile's sum over zeros is not zero.
@@ -237,24 +265,21 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) zeros = O::mfma32(v_operand(vt, c * 16, d), none, zeros);
+        for (int c = 0; c < 4; ++c) zeros = O::mfma32(v_operand(stage, c, d), none, zeros);
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < 16; ++i) bad |= zeros[i] != 0.f;
       poisoned = __ballot(bad) != 0;
     }
     if (!poisoned) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) o[d] = O::mfma32(v_operand(vt, c * 16, d), w[c], o[d]);
+      accumulate(stage, w);
     } else {
       // each key's contribution on its own, added where it is seen
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
-          const typename O::x8 v = v_operand(vt, c * 16, d);
+          const typename O::x8 v = v_operand(stage, c, d);
 #pragma unroll 1
           for (int e = 0; e < 16; ++e) {
             const bool mine = half == e / 8;
@@ -275,6 +300,21 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
         }
     }
   }
+  // then whole tiles, the stage a constant of the code
+  auto step = [&](int stage) __attribute__((always_inline)) {
+    arrive(tile);
+    f32x16 s[2];
+    typename O::x8 w[4];
+    scores_of(stage, s);
+    weights_of(s, w);
+    accumulate(stage, w);
+    --tile;
+  };
+  while (tile > 0) {
+    step(0);
+    step(1);
+  }
+  if (tile == 0) step(0);
 
   if (wave_row + column >= rows) return;
   l = half_sum(l);
