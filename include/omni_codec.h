@@ -1018,7 +1018,9 @@ int omni_read_cache(const omni_kv_cache* cache, const void* slots, int slots_dty
  * type before they meet the values, outputs rounded once.
  *
  * Strides in elements, multiples of 8, at most 2^23 between tokens of k and v; pointers 16-byte aligned;
- * dim a multiple of 8 up to 256; scale positive; out no input. tokens = 0 does nothing.
+ * dim a multiple of 8 up to 256; tokens * heads / kv_heads and key_tokens below 2^31 - 255; scale positive;
+ * out no input. tokens = 0 does nothing. workspace: with
+ * s = omni_prompt_splits(...) above 1, at least s * tokens * heads * (dim + 2) * 4 bytes, 16-byte aligned.
  */
 typedef struct omni_prompt_args {
   const void* q;
@@ -1038,7 +1040,12 @@ typedef struct omni_prompt_args {
   int causal;
   float scale;
   int clear_rest;
+  void* workspace;
+  int64_t workspace_bytes;
 } omni_prompt_args;
+/* In how many pieces, joined in order by a second launch, the keys of a row are taken. */
+int64_t omni_prompt_splits(int64_t tokens, int64_t key_tokens, int64_t sequences, int64_t heads,
+                           int64_t kv_heads);
 int omni_prompt_attention(const omni_prompt_args* args, omni_stream_t stream);
 
 /*

@@ -27,21 +27,23 @@ struct PromptParams {
   const void* starts;
   const void* key_starts;
   int wide;  // the starts are int64
-  int64_t tokens, key_tokens;
+  int tokens, key_tokens;  // tokens * group below 2^31
   int sequences;  // and one past them where the rows behind the last one are cleared
   int cleared;
   int kv_heads, group, dim, causal;
   float scale;  // of the scores, times log2(e)
   int slots;    // row tiles a key head, an upper bound
+  int splits;   // workgroups that share a row tile's keys
+  float* parts;  // with several: [splits][tokens][heads][dim], then [splits][tokens][heads][2] of m and l
 };
 
 constexpr int kKeys = 64;  // of a tile
 constexpr float kLazy = 6.f;
 
-OMNI_DEVICE int64_t start_of(const void* starts, int wide, int64_t at, int64_t end) {
+OMNI_DEVICE int start_of(const void* starts, int wide, int at, int end) {
   const int64_t s = wide ? static_cast<const int64_t*>(starts)[at]
                          : (int64_t) static_cast<const int32_t*>(starts)[at];
-  return s < 0 ? 0 : s > end ? end : s;
+  return (int)(s < 0 ? 0 : s > end ? end : s);
 }
 
 // The LDS slot, of 16 bytes, that piece p of key row r takes in its row: K's rows are read 16 bytes a
@@ -69,56 +71,57 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
   // Key head fastest: the 8 XCDs take workgroups in turn, so with 8 (4, 2) key heads each XCD's L2
   // holds its own head's keys. The last tiles of a sequence, which see the most keys, go first.
   const int kv_head = blockIdx.x % p.kv_heads;
-  const int slot = p.slots - 1 - blockIdx.x / p.kv_heads;
+  const int split = blockIdx.x / p.kv_heads % p.splits;
+  const int slot = p.slots - 1 - blockIdx.x / p.kv_heads / p.splits;
   // Sequence s owns the tiles from floor(first row / kRows) + s on: never fewer than it needs, and
-  // found by search without a sum over the sequences before it.
+  // found by search without a sum over the sequences before it: 64 at a time, each lane one's bounds.
   int lo = 0, n = p.sequences;
-  while (n > 1) {
+  int first, last, key_first, key_last;
+  for (;;) {
     const int step = (n + 63) / 64, at = lane * step;
-    const bool before =
-        at < n && start_of(p.starts, p.wide, lo + at, p.tokens) * p.group / kRows + lo + at <= slot;
-    const int found = __builtin_popcountll(__ballot(before));
-    const int skip = found > 0 ? (found - 1) * step : 0;
-    lo += skip;
-    n = n - skip < step ? n - skip : step;
+    int f = 0, l = 0, kf = 0, kl = 0;
+    if (at < n) {
+      const bool rest = p.cleared && lo + at == p.sequences - 1;  // the rows behind the last sequence
+      f = start_of(p.starts, p.wide, lo + at, p.tokens);
+      l = rest ? p.tokens : start_of(p.starts, p.wide, lo + at + 1, p.tokens);
+      if (!rest) {
+        kf = start_of(p.key_starts, p.wide, lo + at, p.key_tokens);
+        kl = start_of(p.key_starts, p.wide, lo + at + 1, p.key_tokens);
+      }
+    }
+    const bool before = at < n && f * p.group / kRows + lo + at <= slot;
+    const int count = __builtin_popcountll(__ballot(before)), found = count > 0 ? count - 1 : 0;
+    lo += found * step;
+    if (step == 1) {
+      first = __builtin_amdgcn_readlane(f, found);
+      last = __builtin_amdgcn_readlane(l, found);
+      key_first = __builtin_amdgcn_readlane(kf, found);
+      key_last = __builtin_amdgcn_readlane(kl, found);
+      break;
+    }
+    n = n - found * step < step ? n - found * step : step;
   }
-  const int seq = __builtin_amdgcn_readfirstlane(lo);
-  const int64_t first = start_of(p.starts, p.wide, seq, p.tokens);
-  const bool rest = p.cleared && seq == p.sequences - 1;  // the rows behind the last sequence
-  const int64_t last = rest ? p.tokens : start_of(p.starts, p.wide, seq + 1, p.tokens);
-  const int64_t queries = last - first;
-  const int64_t row0 = (slot - (first * p.group / kRows + seq)) * kRows;
-  if (queries <= 0 || row0 < 0 || row0 >= queries * p.group) return;
-  const int64_t key_first = rest ? 0 : start_of(p.key_starts, p.wide, seq, p.key_tokens);
-  int64_t keys = rest ? 0 : start_of(p.key_starts, p.wide, seq + 1, p.key_tokens) - key_first;
-  if (keys < 0) keys = 0;
+  const int queries = last - first, rows = queries * p.group;
+  const int row0 = (slot - (first * p.group / kRows + lo)) * kRows;
+  if (queries <= 0 || row0 < 0 || row0 >= rows) return;
+  const int keys = key_last > key_first ? key_last - key_first : 0;
 
   // this lane's row, and how many keys it, the wave's first and last row and the tile's last see
-  const int64_t wave_row = row0 + wave * 32, rows = queries * p.group;
-  const int64_t row = wave_row + column < rows ? wave_row + column : rows - 1;
-  const int64_t query = row / p.group;
-  const int head = kv_head * p.group + (int)(row - query * p.group);
-  const int64_t ahead = p.causal ? keys - queries + 1 : keys;
-  auto seen_by = [&](int64_t r) {
-    const int64_t s = p.causal ? (r < rows ? r : rows - 1) / p.group + ahead : ahead;
-    return (int)(s < 0 ? 0 : s);
+  const int wave_row = row0 + wave * 32;
+  const int row = wave_row + column < rows ? wave_row + column : rows - 1;
+  const int query = (uint32_t)row / (uint32_t)p.group;
+  const int head = kv_head * p.group + row - query * p.group;
+  const int ahead = p.causal ? keys - queries + 1 : keys;
+  auto seen_by = [&](int r) __attribute__((always_inline)) {
+    const int s = p.causal ? (int)((uint32_t)(r < rows ? r : rows - 1) / (uint32_t)p.group) + ahead : ahead;
+    return s < 0 ? 0 : s;
   };
   const int seen = seen_by(row);
-  const int seen_least = __builtin_amdgcn_readfirstlane(seen_by(wave_row));
-  const int seen_most = wave_row < rows ? __builtin_amdgcn_readfirstlane(seen_by(wave_row + 31)) : 0;
-  const int tiles = (__builtin_amdgcn_readfirstlane(seen_by(row0 + kRows - 1)) + kKeys - 1) / kKeys;
-
-  typename O::x8 q[D / 16];
-  {
-    const uint8_t* from = p.q + (first + query) * p.q_token + head * p.q_head + half * 16;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      if (s * 16 + half * 8 < p.dim)
-        q[s] = *reinterpret_cast<const typename O::x8*>(from + s * 32);
-      else
-        q[s] = typename O::x8{};
-    }
-  }
+  const int seen_least = seen_by(wave_row), seen_most = wave_row < rows ? seen_by(wave_row + 31) : 0;
+  // this workgroup's tiles of them
+  const int all_tiles = (seen_by(row0 + kRows - 1) + kKeys - 1) / kKeys;
+  const int share = (all_tiles + p.splits - 1) / p.splits;
+  const int low = split * share, high = low + share < all_tiles ? low + share : all_tiles;
 
   // DMA: instruction i of the wave fills slots 64 (wave kDma + i) .. of the tile; the row and piece
   // that belong there
@@ -130,15 +133,15 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
     k_off[i] = kp * 8 < p.dim ? (uint32_t)(r * p.k_token + kp * 16) : kOutOfRange;
     v_off[i] = vp * 8 < p.dim ? (uint32_t)(r * p.v_token + vp * 16) : kOutOfRange;
   }
-  const uint8_t* k_base = p.k + key_first * p.k_token + kv_head * p.k_head;
-  const uint8_t* v_base = p.v + key_first * p.v_token + kv_head * p.v_head;
+  const uint8_t* k_base = p.k + (int64_t)key_first * p.k_token + kv_head * p.k_head;
+  const uint8_t* v_base = p.v + (int64_t)key_first * p.v_token + kv_head * p.v_head;
   // rows behind the sequence's last key are zeros
   auto issue = [&](int tile) __attribute__((always_inline)) {
-    const int64_t at = (int64_t)tile * kKeys;
-    const int valid = (int)(keys - at < kKeys ? keys - at : kKeys);
+    const int64_t at = tile * kKeys;
+    const int valid = keys - tile * kKeys < kKeys ? keys - tile * kKeys : kKeys;
     const auto kr = buffer_rsrc(k_base + at * p.k_token, (uint32_t)((valid - 1) * p.k_token + p.dim * 2));
     const auto vr = buffer_rsrc(v_base + at * p.v_token, (uint32_t)((valid - 1) * p.v_token + p.dim * 2));
-    uint8_t* stage = lds + (tile & 1) * 2 * kTile + wave * kDma * 1024;
+    uint8_t* stage = lds + ((tile - low) & 1) * 2 * kTile + wave * kDma * 1024;
 #pragma unroll
     for (int i = 0; i < kDma; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (OMNI_LDS void*)(stage + i * 1024), 16, (int)k_off[i],
@@ -149,6 +152,18 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
                                                (int)v_off[i], 0, 0, 0);
   };
 
+  if (high > low) issue(high - 1);
+  typename O::x8 q[D / 16];
+  {
+    const uint8_t* from = p.q + (int64_t)(first + query) * p.q_token + head * p.q_head + half * 16;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      if (s * 16 + half * 8 < p.dim)
+        q[s] = *reinterpret_cast<const typename O::x8*>(from + s * 32);
+      else
+        q[s] = typename O::x8{};
+    }
+  }
   f32x16 o[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -180,7 +195,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
   auto arrive = [&](int tile) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     asm volatile("s_barrier" ::: "memory");
-    if (tile > 0) issue(tile - 1);
+    if (tile > low) issue(tile - 1);
   };
   auto scores_of = [&](int stage, f32x16 (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -231,14 +246,13 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
       for (int d = 0; d < D / 32; ++d) o[d] = O::mfma32(v_operand(stage, c, d), w[c], o[d]);
   };
 
-  if (tiles > 0) issue(tiles - 1);
   // Tiles from the last: first those that some row of the workgroup does not see whole (and one more
   // where the next would not be in the first stage).
-  int tile = tiles - 1;
-  const int whole = __builtin_amdgcn_readfirstlane(seen_by(row0)) / kKeys;  // tiles that every row sees
-  for (; tile >= 0 && (tile >= whole || tile % 2 == 1); --tile) {
+  int tile = high - 1;
+  const int whole = seen_by(row0) / kKeys;  // tiles that every row sees
+  for (; tile >= low && (tile >= whole || (tile - low) % 2 == 1); --tile) {
     arrive(tile);
-    const int first_key = tile * kKeys, stage = tile & 1;
+    const int first_key = tile * kKeys, stage = (tile - low) & 1;
     if (first_key >= seen_most) continue;
     f32x16 s[2];
     scores_of(stage, s);
@@ -274,30 +288,29 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
     if (!poisoned) {
       accumulate(stage, w);
     } else {
-      // each key's contribution on its own, added where it is seen
+      // each key's contribution on its own, added where it is seen; rare, so a loop of little code
+#pragma unroll 1
+      for (int e = 0; e < kKeys; ++e) {
+        const int c = e / 16, key = first_key + c * 16 + (e % 8 / 4) * 8 + (e % 16 / 8) * 4 + e % 4;
+        const bool mine = half == e % 16 / 8;
+        const typename O::x8 wc = c == 0 ? w[0] : c == 1 ? w[1] : c == 2 ? w[2] : w[3];
+        typename O::x8 we;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+        for (int j = 0; j < 8; ++j) we[j] = mine && j == e % 8 ? wc[j] : (T)0.f;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
           const typename O::x8 v = v_operand(stage, c, d);
-#pragma unroll 1
-          for (int e = 0; e < 16; ++e) {
-            const bool mine = half == e / 8;
-            typename O::x8 ve, we;
+          typename O::x8 ve;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              ve[j] = mine && j == e % 8 ? v[j] : (T)0.f;
-              we[j] = mine && j == e % 8 ? w[c][j] : (T)0.f;
-            }
-            f32x16 part;
+          for (int j = 0; j < 8; ++j) ve[j] = mine && j == e % 8 ? v[j] : (T)0.f;
+          f32x16 part;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) part[i] = 0.f;
-            part = O::mfma32(ve, we, part);
-            const int key = first_key + c * 16 + (e % 8 / 4) * 8 + (e / 8) * 4 + e % 4;
+          for (int i = 0; i < 16; ++i) part[i] = 0.f;
+          part = O::mfma32(ve, we, part);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] += key < seen ? part[i] : 0.f;
-          }
+          for (int i = 0; i < 16; ++i) o[d][i] += key < seen ? part[i] : 0.f;
         }
+      }
     }
   }
   // then whole tiles, the stage a constant of the code
@@ -310,16 +323,35 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
     accumulate(stage, w);
     --tile;
   };
-  while (tile > 0) {
+  while (tile > low) {
     step(0);
     step(1);
   }
-  if (tile == 0) step(0);
+  if (tile == low) step(0);
 
   if (wave_row + column >= rows) return;
   l = half_sum(l);
+  if (p.splits > 1) {
+    const int64_t heads = (int64_t)p.kv_heads * p.group;
+    const int64_t at = ((int64_t)split * p.tokens + first + query) * heads + head;
+    float* stats = p.parts + (int64_t)p.splits * p.tokens * heads * p.dim + at * 2;
+    if (half == 0) {
+      stats[0] = m;
+      stats[1] = l;
+    }
+    if (m == -__builtin_inff()) return;
+    float* to = p.parts + at * p.dim + half * 4;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d * 32 + i * 8 + half * 4 < p.dim)
+          *reinterpret_cast<f32x4*>(to + d * 32 + i * 8) =
+              f32x4{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]};
+    return;
+  }
   const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
-  uint8_t* to = p.out + (first + query) * p.out_token + head * p.out_head + half * 8;
+  uint8_t* to = p.out + (int64_t)(first + query) * p.out_token + head * p.out_head + half * 8;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -332,20 +364,61 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
     }
 }
 
+// The parts of a row's keys joined in their order: 4 dimensions a thread. Rows of no sequence have no
+// parts.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const PromptParams p) {
+  const int quads = p.dim / 4;
+  const int64_t heads = (int64_t)p.kv_heads * p.group, all = p.tokens * heads;
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x, row = item / quads;
+  const int d = (int)(item - row * quads) * 4;
+  if (row >= all) return;
+  const int token = (int)(row / heads);
+  if (token < start_of(p.starts, p.wide, 0, p.tokens) ||
+      (!p.cleared && token >= start_of(p.starts, p.wide, p.sequences, p.tokens)))
+    return;
+  const float* stats = p.parts + p.splits * all * p.dim;
+  float m = -__builtin_inff();
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, stats[(s * all + row) * 2]);
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const float part = stats[(s * all + row) * 2];
+    if (part == -__builtin_inff()) continue;
+    const float keep = __builtin_amdgcn_exp2f(part - m);
+    l = __builtin_fmaf(stats[(s * all + row) * 2 + 1], keep, l);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.parts + (s * all + row) * p.dim + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], keep, o[e]);
+  }
+  const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
+  typename Op<T>::x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * unit);
+  const int head = (int)(row - token * heads);
+  *reinterpret_cast<typename Op<T>::x4*>(p.out + token * p.out_token + head * p.out_head + d * 2) = y;
+}
+
 template <typename T, int D, int NW>
 int launch_prompt(PromptParams p, hipStream_t stream) {
   constexpr int kLds = 2 * 2 * kKeys * D * 2;
-  const int64_t slots = p.tokens * p.group / (32 * NW) + p.sequences;
-  if (slots * p.kv_heads > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+  const int64_t slots = (int64_t)p.tokens * p.group / (32 * NW) + p.sequences;
+  if (slots * p.kv_heads * p.splits > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
   p.slots = (int)slots;
   if (kLds > 64 * 1024) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, D, NW>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
       return OMNI_ERR_LAUNCH;
   }
-  hipLaunchKernelGGL((prompt_kernel<T, D, NW>), dim3((unsigned)(slots * p.kv_heads)), dim3(64 * NW), kLds,
-                     stream, p);
+  hipLaunchKernelGGL((prompt_kernel<T, D, NW>), dim3((unsigned)(slots * p.kv_heads * p.splits)),
+                     dim3(64 * NW), kLds, stream, p);
   OMNI_LAUNCH_CHECK();
+  if (p.splits > 1) {
+    const int64_t items = (int64_t)p.tokens * p.kv_heads * p.group * (p.dim / 4);
+    if ((items + 255) / 256 > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, p);
+    OMNI_LAUNCH_CHECK();
+  }
   return OMNI_OK;
 }
 
@@ -358,6 +431,17 @@ int launch_dim(const PromptParams& p, hipStream_t stream) {
 
 }  // namespace
 
+extern "C" int64_t omni_prompt_splits(int64_t tokens, int64_t key_tokens, int64_t sequences,
+                                      int64_t heads, int64_t kv_heads) {
+  if (tokens < 1 || key_tokens < 1 || heads < 1 || kv_heads < 1 || sequences < 0) return 1;
+  // Row tiles of 128 that leave most of the chip idle share their keys: two workgroups a CU, and four
+  // tiles of keys a workgroup at least.
+  const int64_t workgroups = (tokens * (heads / kv_heads) / 128 + sequences) * kv_heads;
+  const int64_t fill = workgroups > 0 ? 512 / workgroups : 1, most = key_tokens / (4 * kKeys);
+  const int64_t splits = fill < most ? fill : most;
+  return splits < 1 ? 1 : splits > 64 ? 64 : splits;
+}
+
 extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t stream) {
   if (!a || a->tokens < 0 || a->key_tokens < 0 || a->sequences < 0 || a->heads < 1 || a->kv_heads < 1 ||
       a->heads % a->kv_heads || a->heads > 65536 || a->dim < 8 || a->dim % 8 || !(a->scale > 0.f) ||
@@ -365,7 +449,9 @@ extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t st
       (a->dtype != OMNI_DTYPE_BF16 && a->dtype != OMNI_DTYPE_F16) ||
       (a->starts_dtype != OMNI_DTYPE_I32 && a->starts_dtype != OMNI_DTYPE_I64))
     return OMNI_ERR_INVALID_ARG;
-  if (a->dim > 256 || a->key_tokens > 0x7fffff00LL || a->tokens > 0x7fffff00LL) return OMNI_ERR_UNSUPPORTED;
+  if (a->dim > 256 || a->key_tokens > 0x7fffff00LL || a->tokens > 0x7fffff00LL ||
+      a->tokens * (a->heads / a->kv_heads) > 0x7fffff00LL)
+    return OMNI_ERR_UNSUPPORTED;
   const int64_t strides[] = {a->q_stride_token, a->q_stride_head, a->k_stride_token, a->k_stride_head,
                              a->v_stride_token, a->v_stride_head, a->out_stride_token, a->out_stride_head};
   for (int64_t s : strides)
@@ -394,8 +480,8 @@ extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t st
   p.starts = a->starts;
   p.key_starts = a->key_starts;
   p.wide = a->starts_dtype == OMNI_DTYPE_I64;
-  p.tokens = a->tokens;
-  p.key_tokens = a->key_tokens;
+  p.tokens = (int)a->tokens;
+  p.key_tokens = (int)a->key_tokens;
   p.cleared = a->clear_rest ? 1 : 0;
   p.sequences = (int)a->sequences + p.cleared;
   p.kv_heads = (int)a->kv_heads;
@@ -403,6 +489,11 @@ extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t st
   p.dim = (int)a->dim;
   p.causal = a->causal ? 1 : 0;
   p.scale = a->scale * kLog2e;
+  p.splits = (int)omni_prompt_splits(a->tokens, a->key_tokens, a->sequences, a->heads, a->kv_heads);
+  p.parts = static_cast<float*>(a->workspace);
+  if (p.splits > 1 && (!a->workspace || !aligned_to(a->workspace, 16) ||
+                       a->workspace_bytes < p.splits * a->tokens * a->heads * (a->dim + 2) * 4))
+    return OMNI_ERR_INVALID_ARG;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return a->dtype == OMNI_DTYPE_BF16 ? launch_dim<__bf16>(p, s) : launch_dim<_Float16>(p, s);
 }

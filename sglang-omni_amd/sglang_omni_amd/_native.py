@@ -419,6 +419,8 @@ class PromptArgs(ctypes.Structure):
         ("causal", ctypes.c_int),
         ("scale", ctypes.c_float),
         ("clear_rest", ctypes.c_int),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
     ]
 
 
@@ -545,10 +547,11 @@ SIGNATURES: dict[str, list] = {
     "omni_adjust_logits": [ctypes.c_char_p, _PTR],
     "omni_norm_rotary": [ctypes.c_char_p, _PTR],
     "omni_read_cache": [_PTR, _PTR, _INT, _I64, _I64, _PTR, _I64, _I64, _PTR, _I64, _I64, _INT, _PTR],
+    "omni_prompt_splits": [_I64, _I64, _I64, _I64, _I64],
     "omni_prompt_attention": [ctypes.c_char_p, _PTR],
     "omni_paged_attention": [ctypes.c_char_p, _PTR],
 }
-_RESTYPES = {"omni_codec_error_string": ctypes.c_char_p}
+_RESTYPES = {"omni_codec_error_string": ctypes.c_char_p, "omni_prompt_splits": _I64}
 
 _lib: ctypes.CDLL | None = None
 

@@ -13,7 +13,7 @@ _HALVES = (torch.bfloat16, torch.float16)
 _INDEXES = (torch.int64, torch.int32)
 _E4M3 = torch.float8_e4m3fn
 _CODES = N.TORCH_TO_OMNI
-_prompt = None  # the entry points, bound at the first call
+_prompt = _splits = None  # the entry points, bound at the first call
 _paged = None
 
 
@@ -85,14 +85,20 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
         out_token, out_head = _heads(out, "out")
         if out.shape != q.shape or out.dtype is not dtype or out.get_device() != index:
             raise ValueError("out must be like q")
+    sequences = starts.shape[0] - 1
+    global _prompt, _splits
+    if _prompt is None:
+        lib = N.load_library()
+        _prompt, _splits = lib.omni_prompt_attention, lib.omni_prompt_splits
+    splits = _splits(tokens, key_tokens, sequences, heads, kv_heads)
+    needed = splits * tokens * heads * (dim + 2) * 4 if splits > 1 else 0
+    workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
     args = N.pack_prompt(
         q.data_ptr(), q_token, q_head, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head,
         out.data_ptr(), out_token, out_head, _CODES[dtype], tokens, key_tokens, heads, kv_heads, dim,
-        starts.data_ptr(), key_starts.data_ptr(), _CODES[starts.dtype], starts.shape[0] - 1,
-        1 if causal else 0, _scale(scale, dim), 1 if clear else 0)
-    global _prompt
-    if _prompt is None:
-        _prompt = N.load_library().omni_prompt_attention
+        starts.data_ptr(), key_starts.data_ptr(), _CODES[starts.dtype], sequences,
+        1 if causal else 0, _scale(scale, dim), 1 if clear else 0,
+        0 if workspace is None else workspace.data_ptr(), needed)
     status = N.launch_on(index, _prompt, args)
     if status:
         N.check(status, "omni_prompt_attention")
