@@ -1015,12 +1015,13 @@ int omni_read_cache(const omni_kv_cache* cache, const void* slots, int slots_dty
  * sees none, or whose scores are all -infinity, is zero; values behind what a query sees do not reach
  * it, whatever they hold. Rows of out outside the sequences stay as they are; with clear_rest those
  * from starts[sequences] on become zero. Scores, maxima and sums float32, softmax weights rounded to the
- * type before they meet the values, outputs rounded once.
+ * type before they meet the values, outputs rounded once. How the keys of a row are divided over waves
+ * and workgroups follows from the call's sizes, so the last bits of a row may depend on what else is in it.
  *
  * Strides in elements, multiples of 8, at most 2^23 between tokens of k and v; pointers 16-byte aligned;
  * dim a multiple of 8 up to 256; tokens * heads / kv_heads and key_tokens below 2^31 - 255; scale positive;
  * out no input. tokens = 0 does nothing. workspace: with
- * s = omni_prompt_splits(...) above 1, at least s * tokens * heads * (dim + 2) * 4 bytes, 16-byte aligned.
+ * s = omni_prompt_plan(...) above 1, at least s * tokens * heads * (dim + 2) * 4 bytes, 16-byte aligned.
  */
 typedef struct omni_prompt_args {
   const void* q;
@@ -1043,9 +1044,10 @@ typedef struct omni_prompt_args {
   void* workspace;
   int64_t workspace_bytes;
 } omni_prompt_args;
-/* In how many pieces, joined in order by a second launch, the keys of a row are taken. */
-int64_t omni_prompt_splits(int64_t tokens, int64_t key_tokens, int64_t sequences, int64_t heads,
-                           int64_t kv_heads);
+/* In how many pieces, joined in order by a second launch, the keys of a row are taken, and (unless null)
+ * the rows of a workgroup, 32 or 128. */
+int64_t omni_prompt_plan(int64_t tokens, int64_t key_tokens, int64_t sequences, int64_t heads,
+                         int64_t kv_heads, int64_t dim, int causal, int* tile_rows);
 int omni_prompt_attention(const omni_prompt_args* args, omni_stream_t stream);
 
 /*

@@ -14,6 +14,8 @@
 // .. 11, the others 4 .. 7 and 12 .. 15, and V^T, read transposed, takes its keys in that order. The
 // weights are rounded to the rows' type for that product (half a step of each, the sum l is of the
 // unrounded ones); scores, maxima, sums and outputs are float32.
+#include <type_traits>
+
 #include "attention.h"
 
 namespace {
@@ -37,8 +39,8 @@ struct PromptParams {
   float* parts;  // with several: [splits][tokens][heads][dim], then [splits][tokens][heads][2] of m and l
 };
 
-constexpr int kKeys = 64;  // of a tile
 constexpr float kLazy = 6.f;
+constexpr int keys_of(int dim, bool long_form) { return long_form && dim < 256 ? 64 : 32; }  // of a tile
 
 OMNI_DEVICE int start_of(const void* starts, int wide, int at, int end) {
   const int64_t s = wide ? static_cast<const int64_t*>(starts)[at]
@@ -57,14 +59,21 @@ OMNI_DEVICE int v_slot(int r, int p) {
   return D == 64 ? p ^ (((r >> 1) & 1) * 4) : p ^ ((r & 3) * 4);
 }
 
-template <typename T, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const PromptParams p) {
+//
+// LONG: the waves own 32 rows each and share the tiles, [2][K, V] in shared memory, the next one on its
+// way. Not LONG, for few rows: the waves share 32 rows and each owns every NW-th tile, [NW][K, V], and
+// their parts are joined at the end; so many more workgroups, each with fewer tiles one after the other.
+template <typename T, int D, int NW, bool LONG>
+__global__ void __launch_bounds__(64 * NW, D < 256 ? 2 : 1) prompt_kernel(const PromptParams p) {
   using O = Op<T>;
-  constexpr int kRows = 32 * NW;
+  constexpr int kRows = LONG ? 32 * NW : 32;
+  constexpr int kKeys = keys_of(D, LONG), kBlocks = kKeys / 32, kSteps = kKeys / 16;
   constexpr int kPieces = D / 8;  // 16-byte pieces of a row
   constexpr int kTile = kKeys * D * 2;
-  constexpr int kDma = kKeys * kPieces / 64 / NW;  // instructions a wave and tile
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2][K, V]
+  // DMA instructions a wave and tile; their offsets repeat after 16 rows
+  constexpr int kDma = kKeys * kPieces / 64 / (LONG ? NW : 1);
+  constexpr int kOffsets = LONG ? kDma : kDma / kSteps;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, half = lane >> 5, column = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 
@@ -107,7 +116,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
   const int keys = key_last > key_first ? key_last - key_first : 0;
 
   // this lane's row, and how many keys it, the wave's first and last row and the tile's last see
-  const int wave_row = row0 + wave * 32;
+  const int wave_row = row0 + (LONG ? wave * 32 : 0);
   const int row = wave_row + column < rows ? wave_row + column : rows - 1;
   const int query = (uint32_t)row / (uint32_t)p.group;
   const int head = kv_head * p.group + row - query * p.group;
@@ -123,12 +132,12 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
   const int share = (all_tiles + p.splits - 1) / p.splits;
   const int low = split * share, high = low + share < all_tiles ? low + share : all_tiles;
 
-  // DMA: instruction i of the wave fills slots 64 (wave kDma + i) .. of the tile; the row and piece
-  // that belong there
-  uint32_t k_off[kDma], v_off[kDma];
+  // DMA: instruction i of the wave fills slots 64 i .. of its part of the tile; the row and piece that
+  // belong there
+  uint32_t k_off[kOffsets], v_off[kOffsets];
 #pragma unroll
-  for (int i = 0; i < kDma; ++i) {
-    const int at = (wave * kDma + i) * 64 + lane, r = at / kPieces, s = at % kPieces;
+  for (int i = 0; i < kOffsets; ++i) {
+    const int at = ((LONG ? wave * kDma : 0) + i) * 64 + lane, r = at / kPieces, s = at % kPieces;
     const int kp = k_slot<D>(r, s), vp = v_slot<D>(r, s);
     k_off[i] = kp * 8 < p.dim ? (uint32_t)(r * p.k_token + kp * 16) : kOutOfRange;
     v_off[i] = vp * 8 < p.dim ? (uint32_t)(r * p.v_token + vp * 16) : kOutOfRange;
@@ -136,23 +145,28 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
   const uint8_t* k_base = p.k + (int64_t)key_first * p.k_token + kv_head * p.k_head;
   const uint8_t* v_base = p.v + (int64_t)key_first * p.v_token + kv_head * p.v_head;
   // rows behind the sequence's last key are zeros
+  auto issue_rows = [&](const uint8_t* base, int64_t pitch, const uint32_t (&off)[kOffsets], int tile,
+                        uint32_t stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < kDma / kOffsets; ++g) {
+      const int at = tile * kKeys + g * 16;
+      const int valid = keys - at < kKeys ? keys - at : kKeys;
+      const u32x4 rsrc =
+          dma_rsrc(base + at * pitch, valid > 0 ? (uint32_t)((valid - 1) * pitch + p.dim * 2) : 0u);
+#pragma unroll
+      for (int i = 0; i < kOffsets; ++i) dma_rows(rsrc, stage + (g * kOffsets + i) * 1024, off[i]);
+    }
+  };
+  const uint32_t place =
+      (uint32_t)(uintptr_t)(OMNI_LDS uint8_t*)lds + (LONG ? wave * kDma * 1024 : wave * 2 * kTile);
   auto issue = [&](int tile) __attribute__((always_inline)) {
-    const int64_t at = tile * kKeys;
-    const int valid = keys - tile * kKeys < kKeys ? keys - tile * kKeys : kKeys;
-    const auto kr = buffer_rsrc(k_base + at * p.k_token, (uint32_t)((valid - 1) * p.k_token + p.dim * 2));
-    const auto vr = buffer_rsrc(v_base + at * p.v_token, (uint32_t)((valid - 1) * p.v_token + p.dim * 2));
-    uint8_t* stage = lds + ((tile - low) & 1) * 2 * kTile + wave * kDma * 1024;
-#pragma unroll
-    for (int i = 0; i < kDma; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (OMNI_LDS void*)(stage + i * 1024), 16, (int)k_off[i],
-                                               0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < kDma; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (OMNI_LDS void*)(stage + kTile + i * 1024), 16,
-                                               (int)v_off[i], 0, 0, 0);
+    const uint32_t stage = place + (LONG ? ((tile - low) & 1) * 2 * kTile : 0);
+    issue_rows(k_base, p.k_token, k_off, tile, stage);
+    issue_rows(v_base, p.v_token, v_off, tile, stage + kTile);
   };
 
-  if (high > low) issue(high - 1);
+  const int top_tile = high - 1 - (LONG ? 0 : wave);
+  if (top_tile >= low) issue(top_tile);
   typename O::x8 q[D / 16];
   {
     const uint8_t* from = p.q + (int64_t)(first + query) * p.q_token + head * p.q_head + half * 16;
@@ -182,7 +196,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
     const int r = half * 4 + ((lane & 15) >> 2), piece = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
     v_at[d] = kTile + r * kPitch + v_slot<D>(r, piece) * 16 + (lane & 1) * 8;
   }
-  const uint8_t OMNI_LDS* shared = (const uint8_t OMNI_LDS*)lds;
+  const uint8_t OMNI_LDS* shared = (const uint8_t OMNI_LDS*)lds + (LONG ? 0 : wave * 2 * kTile);
   auto k_operand = [&](int stage, int b, int c) __attribute__((always_inline)) {
     return *(const typename O::x8 OMNI_LDS*)(shared + k_at[c] + (stage * 2 * kTile + b * 32 * kPitch));
   };
@@ -197,23 +211,23 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
     asm volatile("s_barrier" ::: "memory");
     if (tile > low) issue(tile - 1);
   };
-  auto scores_of = [&](int stage, f32x16 (&s)[2]) __attribute__((always_inline)) {
+  auto scores_of = [&](int stage, f32x16 (&s)[kBlocks]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) s[b] = O::mfma32(k_operand(stage, b, c), q[c], s[b]);
+      for (int b = 0; b < kBlocks; ++b) s[b] = O::mfma32(k_operand(stage, b, c), q[c], s[b]);
   };
   // The weights of a tile's scores. The maximum they are taken against moves only where a score is past
   // it by more than 2^kLazy: until then weights are that much larger, which costs no precision, and the
   // sums and outputs need no rescaling.
-  auto weights_of = [&](const f32x16 (&s)[2], typename O::x8 (&w)[4]) __attribute__((always_inline)) {
+  auto weights_of = [&](const f32x16 (&s)[kBlocks], typename O::x8 (&w)[kSteps]) __attribute__((always_inline)) {
     float top = s[0][0];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = half_max(top) * p.scale;
@@ -231,7 +245,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
     }
     const float shift = O::kBias - m_use;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], p.scale, shift));
@@ -239,129 +253,203 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(const
         w[b * 2 + i / 8][i % 8] = (T)x;
       }
   };
-  auto accumulate = [&](int stage, const typename O::x8 (&w)[4]) __attribute__((always_inline)) {
+  auto accumulate = [&](int stage, const typename O::x8 (&w)[kSteps]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < kSteps; ++c)
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) o[d] = O::mfma32(v_operand(stage, c, d), w[c], o[d]);
   };
 
-  // Tiles from the last: first those that some row of the workgroup does not see whole (and one more
-  // where the next would not be in the first stage).
-  int tile = high - 1;
-  const int whole = seen_by(row0) / kKeys;  // tiles that every row sees
-  for (; tile >= low && (tile >= whole || (tile - low) % 2 == 1); --tile) {
-    arrive(tile);
-    const int first_key = tile * kKeys, stage = (tile - low) & 1;
-    if (first_key >= seen_most) continue;
-    f32x16 s[2];
-    scores_of(stage, s);
-    const bool partial = first_key + kKeys > seen_least;
-    bool poisoned = false;
-    if (partial) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = first_key + b * 32 + (i / 4) * 8 + half * 4 + i % 4;
-          s[b][i] = key < seen ? s[b][i] : -__builtin_inff();
-        }
+  // 4 dimensions of a row, from d on, out: the result, or where workgroups share the keys a part (without
+  // keys of its own its maximum alone)
+  auto store_row = [&](int at_query, int at_head, int d, f32x4 x, float m, float l)
+                       __attribute__((always_inline)) {
+    const int64_t token = first + at_query;
+    if (p.splits > 1) {
+      const int64_t heads = (int64_t)p.kv_heads * p.group, at = ((int64_t)split * p.tokens + token) * heads + at_head;
+      if (d == 0) {
+        float* stats = p.parts + (int64_t)p.splits * p.tokens * heads * p.dim + at * 2;
+        stats[0] = m;
+        stats[1] = l;
+      }
+      if (m != -__builtin_inff()) *reinterpret_cast<f32x4*>(p.parts + at * p.dim + d) = x;
+      return;
     }
-    typename O::x8 w[4];
-    weights_of(s, w);
-    if (partial) {
-      // A key that some of these rows do not see may hold an infinity or a NaN, and zero times it is
-      // one too: such a tile's sum over zeros is not zero.
-      f32x16 zeros;
+    const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
+    typename O::x4 y;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) zeros[i] = 0.f;
-      const typename O::x8 none{};
+    for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * unit);
+    *reinterpret_cast<typename O::x4*>(p.out + token * p.out_token + at_head * p.out_head + d * 2) = y;
+  };
+  // what a row does not see: its scores
+  auto hide = [&](int first_key, f32x16 (&s)[kBlocks]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d)
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) zeros = O::mfma32(v_operand(stage, c, d), none, zeros);
-      bool bad = false;
+      for (int i = 0; i < 16; ++i) {
+        const int key = first_key + b * 32 + (i / 4) * 8 + half * 4 + i % 4;
+        s[b][i] = key < seen ? s[b][i] : -__builtin_inff();
+      }
+  };
+  // and its values: one that some of these rows do not see may be an infinity or a NaN, and zero times
+  // it is one too. Such a tile's sum over zeros is not zero.
+  auto accumulate_seen = [&](int first_key, int stage, const typename O::x8 (&w)[kSteps])
+                             __attribute__((always_inline)) {
+    f32x16 zeros;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) bad |= zeros[i] != 0.f;
-      poisoned = __ballot(bad) != 0;
-    }
-    if (!poisoned) {
+    for (int i = 0; i < 16; ++i) zeros[i] = 0.f;
+    const typename O::x8 none{};
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) zeros = O::mfma32(v_operand(stage, c, d), none, zeros);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad |= zeros[i] != 0.f;
+    if (__ballot(bad) == 0) {
       accumulate(stage, w);
-    } else {
-      // each key's contribution on its own, added where it is seen; rare, so a loop of little code
+      return;
+    }
+    // each key's contribution on its own, added where it is seen; rare, so a loop of little code
 #pragma unroll 1
-      for (int e = 0; e < kKeys; ++e) {
-        const int c = e / 16, key = first_key + c * 16 + (e % 8 / 4) * 8 + (e % 16 / 8) * 4 + e % 4;
-        const bool mine = half == e % 16 / 8;
-        const typename O::x8 wc = c == 0 ? w[0] : c == 1 ? w[1] : c == 2 ? w[2] : w[3];
-        typename O::x8 we;
+    for (int e = 0; e < kKeys; ++e) {
+      const int c = e / 16, key = first_key + c * 16 + (e % 8 / 4) * 8 + (e % 16 / 8) * 4 + e % 4;
+      const bool mine = half == e % 16 / 8;
+      typename O::x8 wc = w[0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) we[j] = mine && j == e % 8 ? wc[j] : (T)0.f;
+      for (int i = 1; i < kSteps; ++i) wc = c == i ? w[i] : wc;
+      typename O::x8 we;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          const typename O::x8 v = v_operand(stage, c, d);
-          typename O::x8 ve;
+      for (int j = 0; j < 8; ++j) we[j] = mine && j == e % 8 ? wc[j] : (T)0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ve[j] = mine && j == e % 8 ? v[j] : (T)0.f;
-          f32x16 part;
+      for (int d = 0; d < D / 32; ++d) {
+        const typename O::x8 v = v_operand(stage, c, d);
+        typename O::x8 ve;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[i] = 0.f;
-          part = O::mfma32(ve, we, part);
+        for (int j = 0; j < 8; ++j) ve[j] = mine && j == e % 8 ? v[j] : (T)0.f;
+        f32x16 part;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[d][i] += key < seen ? part[i] : 0.f;
-        }
+        for (int i = 0; i < 16; ++i) part[i] = 0.f;
+        part = O::mfma32(ve, we, part);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] += key < seen ? part[i] : 0.f;
       }
     }
-  }
-  // then whole tiles, the stage a constant of the code
-  auto step = [&](int stage) __attribute__((always_inline)) {
-    arrive(tile);
-    f32x16 s[2];
-    typename O::x8 w[4];
-    scores_of(stage, s);
-    weights_of(s, w);
-    accumulate(stage, w);
-    --tile;
   };
-  while (tile > low) {
-    step(0);
-    step(1);
-  }
-  if (tile == low) step(0);
 
-  if (wave_row + column >= rows) return;
-  l = half_sum(l);
-  if (p.splits > 1) {
-    const int64_t heads = (int64_t)p.kv_heads * p.group;
-    const int64_t at = ((int64_t)split * p.tokens + first + query) * heads + head;
-    float* stats = p.parts + (int64_t)p.splits * p.tokens * heads * p.dim + at * 2;
-    if (half == 0) {
-      stats[0] = m;
-      stats[1] = l;
+  if constexpr (LONG) {
+    // Tiles from the last: first those that some row of the workgroup does not see whole (and one more
+    // where the next would not be in the first stage).
+    int tile = high - 1;
+    const int whole = seen_by(row0) / kKeys;  // tiles that every row sees
+    for (; tile >= low && (tile >= whole || (tile - low) % 2 == 1); --tile) {
+      arrive(tile);
+      const int first_key = tile * kKeys, stage = (tile - low) & 1;
+      if (first_key >= seen_most) continue;
+      const bool partial = first_key + kKeys > seen_least;
+      f32x16 s[kBlocks];
+      typename O::x8 w[kSteps];
+      scores_of(stage, s);
+      if (partial) hide(first_key, s);
+      weights_of(s, w);
+      if (partial)
+        accumulate_seen(first_key, stage, w);
+      else
+        accumulate(stage, w);
     }
-    if (m == -__builtin_inff()) return;
-    float* to = p.parts + at * p.dim + half * 4;
+    // then whole tiles, the stage a constant of the code
+    auto step = [&](int stage) __attribute__((always_inline)) {
+      arrive(tile);
+      f32x16 s[kBlocks];
+      typename O::x8 w[kSteps];
+      scores_of(stage, s);
+      weights_of(s, w);
+      accumulate(stage, w);
+      --tile;
+    };
+    while (tile > low) {
+      step(0);
+      step(1);
+    }
+    if (tile == low) step(0);
+  } else {
+    int tile = top_tile;
+    auto step = [&](auto partial) __attribute__((always_inline)) {
+      const int first_key = tile * kKeys;
+      f32x16 s[kBlocks];
+      typename O::x8 w[kSteps];
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");  // K is here, V may be on its way
+      scores_of(0, s);
+      // once K has been read, the next one takes its place, and below so for V
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (tile - NW >= low) issue_rows(k_base, p.k_token, k_off, tile - NW, place);
+      if constexpr (partial) hide(first_key, s);
+      weights_of(s, w);
+      if (tile - NW >= low)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if constexpr (partial)
+        accumulate_seen(first_key, 0, w);
+      else
+        accumulate(0, w);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (tile - NW >= low) issue_rows(v_base, p.v_token, v_off, tile - NW, place + kTile);
+      tile -= NW;
+    };
+    while (tile >= low && tile * kKeys + kKeys > seen_least) step(std::true_type{});
+    while (tile >= low) step(std::false_type{});
+    // The waves' parts joined: each leaves its outputs in its own tiles' place, and a thread takes 4
+    // dimensions of a row from all of them, in their order.
+    constexpr int kLine = D;  // floats
+    static_assert(32 * kLine * 4 <= 2 * kTile, "a wave's outputs fit its tiles");
+    float* const stats = reinterpret_cast<float*>(lds + NW * 2 * kTile);  // [NW][2][32]
+    auto place_of = [](int r, int quad) { return r * kLine + (quad ^ (r & 7)) * 4; };
+    l = half_sum(l);
+    if (half == 0) {
+      stats[wave * 64 + column] = m;
+      stats[wave * 64 + 32 + column] = l;
+    }
+    float* const mine = reinterpret_cast<float*>(lds + wave * 2 * kTile);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (d * 32 + i * 8 + half * 4 < p.dim)
-          *reinterpret_cast<f32x4*>(to + d * 32 + i * 8) =
-              f32x4{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]};
+        *reinterpret_cast<f32x4*>(mine + place_of(column, d * 8 + i * 2 + half)) =
+            f32x4{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]};
+    __syncthreads();
+    for (int item = threadIdx.x; item < 32 * (D / 4); item += 64 * NW) {
+      const int r = item / (D / 4), d = item % (D / 4) * 4;
+      if (row0 + r >= rows || d >= p.dim) continue;
+      float m_all = stats[r];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) m_all = fmaxf(m_all, stats[w * 64 + r]);
+      const float m_base = m_all == -__builtin_inff() ? 0.f : m_all;
+      float l_all = 0.f;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float keep = __builtin_amdgcn_exp2f(stats[w * 64 + r] - m_base);
+        l_all = __builtin_fmaf(stats[w * 64 + 32 + r], keep, l_all);
+        const f32x4 part = *reinterpret_cast<const f32x4*>(lds + w * 2 * kTile + place_of(r, d / 4) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(part[e], keep, x[e]);
+      }
+      const int at_query = (uint32_t)(row0 + r) / (uint32_t)p.group;
+      store_row(at_query, kv_head * p.group + row0 + r - at_query * p.group, d, x, m_all, l_all);
+    }
     return;
   }
-  const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
-  uint8_t* to = p.out + (int64_t)(first + query) * p.out_token + head * p.out_head + half * 8;
+
+  if (wave_row + column >= rows) return;
+  l = half_sum(l);
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (d * 32 + i * 8 + half * 4 >= p.dim) continue;
-      typename O::x4 x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (T)(o[d][i * 4 + j] * unit);
-      *reinterpret_cast<typename O::x4*>(to + d * 64 + i * 16) = x;
-    }
+    for (int i = 0; i < 4; ++i)
+      if (d * 32 + i * 8 + half * 4 < p.dim)
+        store_row(query, head, d * 32 + i * 8 + half * 4,
+                  f32x4{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]}, m, l);
 }
 
 // The parts of a row's keys joined in their order: 4 dimensions a thread. Rows of no sequence have no
@@ -399,18 +487,19 @@ __global__ void __launch_bounds__(256) join_kernel(const PromptParams p) {
   *reinterpret_cast<typename Op<T>::x4*>(p.out + token * p.out_token + head * p.out_head + d * 2) = y;
 }
 
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, bool LONG>
 int launch_prompt(PromptParams p, hipStream_t stream) {
-  constexpr int kLds = 2 * 2 * kKeys * D * 2;
-  const int64_t slots = (int64_t)p.tokens * p.group / (32 * NW) + p.sequences;
+  constexpr int kTiles = 2 * keys_of(D, LONG) * D * 2;
+  constexpr int kLds = LONG ? 2 * kTiles : NW * (kTiles + 64 * 4);
+  const int64_t slots = (int64_t)p.tokens * p.group / (LONG ? 32 * NW : 32) + p.sequences;
   if (slots * p.kv_heads * p.splits > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
   p.slots = (int)slots;
   if (kLds > 64 * 1024) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, D, NW>),
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, D, NW, LONG>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
       return OMNI_ERR_LAUNCH;
   }
-  hipLaunchKernelGGL((prompt_kernel<T, D, NW>), dim3((unsigned)(slots * p.kv_heads * p.splits)),
+  hipLaunchKernelGGL((prompt_kernel<T, D, NW, LONG>), dim3((unsigned)(slots * p.kv_heads * p.splits)),
                      dim3(64 * NW), kLds, stream, p);
   OMNI_LAUNCH_CHECK();
   if (p.splits > 1) {
@@ -422,24 +511,69 @@ int launch_prompt(PromptParams p, hipStream_t stream) {
   return OMNI_OK;
 }
 
+struct Plan {
+  bool long_form;
+  int splits;
+};
+
+// The form and the number of workgroups that share a row tile's keys: the least of their estimated times
+// in us, which come from what the host knows, so with sequences taken to be of one length. Of each form:
+// a workgroup's start and end on a CU that others share, its time a step (64 keys of 128 rows, or 128 of
+// 32) there, and a step's time in a chain of them. Fitted to 37 .. 8192 tokens of 8 .. 32 heads alone and
+// in batches, and 1 .. 1000 tokens after 4000 .. 100000 keys; the choice is the fastest measured one or
+// within 20 % of it. 1000 tokens of 16 heads over 8: 15.7 us not LONG, 26.3 LONG; 8192 of them 370 and
+// 292; 500 tokens of 32 heads after 20000 keys 218 not LONG, 391 LONG, 175 LONG in four pieces.
+Plan plan_of(int64_t tokens, int64_t key_tokens, int64_t sequences, int64_t heads, int64_t kv_heads,
+             int64_t dim, bool causal) {
+  struct Cost {
+    double start, step, chain;
+  };
+  constexpr Cost kCosts[3][2] = {{{1.8, 0.36, 0.6}, {3.0, 0.52, 0.83}},
+                                 {{3.0, 0.72, 0.9}, {4.0, 0.97, 1.1}},
+                                 {{6.0, 1.8, 1.8}, {8.0, 3.1, 3.2}}};
+  const Cost* costs = kCosts[dim <= 64 ? 0 : dim <= 128 ? 1 : 2];
+  const double count = sequences > 0 ? (double)sequences : 1.0;
+  const double keys = key_tokens / count, queries = tokens / count;
+  const double seen = causal ? (queries < keys ? keys - queries / 2 : keys / 2) : keys;
+  const double rows = (double)tokens * (heads / kv_heads);
+  Plan best = {false, 1};
+  double least = 1e30;
+  for (int form = 0; form < 2; ++form) {
+    const double tiles = (rows / (form ? 128 : 32) + count) * kv_heads, width = form ? 64 : 128;
+    for (int splits = 1; splits <= 32 && (splits == 1 || keys >= 256.0 * splits); splits *= 2) {
+      const double busy = tiles * splits / 256;
+      const double shared = busy * (costs[form].start + costs[form].step * seen / width / splits);
+      const double alone = keys / width / splits * costs[form].chain * (form && busy > 1 ? 1.4 : 1.0);
+      const double parts = (double)tokens * heads * (dim + 2) * 8 * splits;  // bytes there and back
+      const double joined = splits > 1 ? 6 + 0.4 * splits + parts / 4e6 : 0;
+      const double time = (form ? 1.0 : 0.0) + (shared > alone ? shared : alone) + joined;
+      if (time < least) {
+        least = time;
+        best = {form == 1, splits};
+      }
+    }
+  }
+  return best;
+}
+
 template <typename T>
-int launch_dim(const PromptParams& p, hipStream_t stream) {
-  if (p.dim <= 64) return launch_prompt<T, 64, 4>(p, stream);
-  if (p.dim <= 128) return launch_prompt<T, 128, 4>(p, stream);
-  return launch_prompt<T, 256, 4>(p, stream);
+int launch_dim(const PromptParams& p, bool long_form, hipStream_t stream) {
+  if (p.dim <= 64)
+    return long_form ? launch_prompt<T, 64, 4, true>(p, stream) : launch_prompt<T, 64, 4, false>(p, stream);
+  if (p.dim <= 128)
+    return long_form ? launch_prompt<T, 128, 4, true>(p, stream) : launch_prompt<T, 128, 4, false>(p, stream);
+  return long_form ? launch_prompt<T, 256, 4, true>(p, stream) : launch_prompt<T, 256, 4, false>(p, stream);
 }
 
 }  // namespace
 
-extern "C" int64_t omni_prompt_splits(int64_t tokens, int64_t key_tokens, int64_t sequences,
-                                      int64_t heads, int64_t kv_heads) {
-  if (tokens < 1 || key_tokens < 1 || heads < 1 || kv_heads < 1 || sequences < 0) return 1;
-  // Row tiles of 128 that leave most of the chip idle share their keys: two workgroups a CU, and four
-  // tiles of keys a workgroup at least.
-  const int64_t workgroups = (tokens * (heads / kv_heads) / 128 + sequences) * kv_heads;
-  const int64_t fill = workgroups > 0 ? 512 / workgroups : 1, most = key_tokens / (4 * kKeys);
-  const int64_t splits = fill < most ? fill : most;
-  return splits < 1 ? 1 : splits > 64 ? 64 : splits;
+extern "C" int64_t omni_prompt_plan(int64_t tokens, int64_t key_tokens, int64_t sequences, int64_t heads,
+                                    int64_t kv_heads, int64_t dim, int causal, int* tile_rows) {
+  Plan plan = {false, 1};
+  if (tokens > 0 && key_tokens > 0 && heads > 0 && kv_heads > 0 && sequences >= 0)
+    plan = plan_of(tokens, key_tokens, sequences, heads, kv_heads, dim, causal != 0);
+  if (tile_rows) *tile_rows = plan.long_form ? 128 : 32;
+  return plan.splits;
 }
 
 extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t stream) {
@@ -489,11 +623,14 @@ extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t st
   p.dim = (int)a->dim;
   p.causal = a->causal ? 1 : 0;
   p.scale = a->scale * kLog2e;
-  p.splits = (int)omni_prompt_splits(a->tokens, a->key_tokens, a->sequences, a->heads, a->kv_heads);
+  int tile_rows;
+  p.splits = (int)omni_prompt_plan(a->tokens, a->key_tokens, a->sequences, a->heads, a->kv_heads, a->dim,
+                                   a->causal, &tile_rows);
   p.parts = static_cast<float*>(a->workspace);
   if (p.splits > 1 && (!a->workspace || !aligned_to(a->workspace, 16) ||
                        a->workspace_bytes < p.splits * a->tokens * a->heads * (a->dim + 2) * 4))
     return OMNI_ERR_INVALID_ARG;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return a->dtype == OMNI_DTYPE_BF16 ? launch_dim<__bf16>(p, s) : launch_dim<_Float16>(p, s);
+  return a->dtype == OMNI_DTYPE_BF16 ? launch_dim<__bf16>(p, tile_rows == 128, s)
+                                     : launch_dim<_Float16>(p, tile_rows == 128, s);
 }

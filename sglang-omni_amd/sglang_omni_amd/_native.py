@@ -547,11 +547,11 @@ SIGNATURES: dict[str, list] = {
     "omni_adjust_logits": [ctypes.c_char_p, _PTR],
     "omni_norm_rotary": [ctypes.c_char_p, _PTR],
     "omni_read_cache": [_PTR, _PTR, _INT, _I64, _I64, _PTR, _I64, _I64, _PTR, _I64, _I64, _INT, _PTR],
-    "omni_prompt_splits": [_I64, _I64, _I64, _I64, _I64],
+    "omni_prompt_plan": [_I64, _I64, _I64, _I64, _I64, _I64, _INT, ctypes.POINTER(_INT)],
     "omni_prompt_attention": [ctypes.c_char_p, _PTR],
     "omni_paged_attention": [ctypes.c_char_p, _PTR],
 }
-_RESTYPES = {"omni_codec_error_string": ctypes.c_char_p, "omni_prompt_splits": _I64}
+_RESTYPES = {"omni_codec_error_string": ctypes.c_char_p, "omni_prompt_plan": _I64}
 
 _lib: ctypes.CDLL | None = None
 

@@ -13,7 +13,7 @@ _HALVES = (torch.bfloat16, torch.float16)
 _INDEXES = (torch.int64, torch.int32)
 _E4M3 = torch.float8_e4m3fn
 _CODES = N.TORCH_TO_OMNI
-_prompt = _splits = None  # the entry points, bound at the first call
+_prompt = _plan = None  # the entry points, bound at the first call
 _paged = None
 
 
@@ -52,7 +52,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     may be the last piece of a longer sequence. A query that sees no key (or whose scores are all
     -infinity) is zero, and what lies behind a query's keys does not reach it, not even as NaN. scale
     defaults to dim ** -0.5. Softmax weights are rounded to the type before they meet the values, as the
-    matrix cores take them; all sums are float32 and the output is rounded once.
+    matrix cores take them; all sums are float32 and the output is rounded once. How a row's keys are
+    divided over the chip follows from the call's sizes, and with it the row's last bits.
 
     bf16 or f16; dim a multiple of 8 up to 256; heads contiguous and 16-byte aligned, other strides free.
     Rows of ``out`` behind the last sequence stay as they are; those of an output made here are zero."""
@@ -86,11 +87,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
         if out.shape != q.shape or out.dtype is not dtype or out.get_device() != index:
             raise ValueError("out must be like q")
     sequences = starts.shape[0] - 1
-    global _prompt, _splits
+    global _prompt, _plan
     if _prompt is None:
         lib = N.load_library()
-        _prompt, _splits = lib.omni_prompt_attention, lib.omni_prompt_splits
-    splits = _splits(tokens, key_tokens, sequences, heads, kv_heads)
+        _prompt, _plan = lib.omni_prompt_attention, lib.omni_prompt_plan
+    splits = _plan(tokens, key_tokens, sequences, heads, kv_heads, dim, 1 if causal else 0, None)
     needed = splits * tokens * heads * (dim + 2) * 4 if splits > 1 else 0
     workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
     args = N.pack_prompt(

@@ -116,6 +116,31 @@ def test_one_long_sequence(gpu):
     check(q[:100], k, v, [100], [3001])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("lengths,before,heads,kv,rows,split", [
+    ([700, 650], 0, 64, 16, 128, False), ([300], 0, 4, 2, 32, False), ([500], 15000, 32, 4, 128, True),
+    ([3], 6000, 4, 2, 32, True), ([9, 0, 31], 3000, 8, 2, 32, True)])
+def test_every_form(gpu, dtype, dim, lengths, before, heads, kv, rows, split):
+    """Rows of a workgroup 32 or 128, the keys of a row in one piece or several."""
+    key_lengths = [n + before for n in lengths]
+    tile = N.ctypes.c_int()
+    pieces = N.load_library().omni_prompt_plan(sum(lengths), sum(key_lengths), len(lengths), heads, kv, dim,
+                                               1, N.ctypes.byref(tile))
+    assert (pieces > 1) == split and tile.value == rows
+    g = torch.Generator().manual_seed(dim + before)
+    q = random_heads(g, sum(lengths), heads, dim, dtype, gpu, 2.0)
+    k, v = (random_heads(g, sum(key_lengths), kv, dim, dtype, gpu) for _ in range(2))
+    check(q, k, v, lengths, key_lengths)
+    # rows behind the last sequence, and a sequence whose queries see nothing
+    few = [lengths[0], *lengths[1:-1], lengths[-1] - 2] if lengths[-1] > 2 else lengths
+    got = check(q, k, v, few, key_lengths)
+    assert (got[sum(few):] == 0).all()
+    out = torch.full_like(q, 7.0)
+    prompt_attention(q, k, v, starts_of(few, gpu), key_starts=starts_of(key_lengths, gpu), out=out)
+    assert torch.equal(out[:sum(few)], got[:sum(few)]) and (out[sum(few):] == 7).all()
+
+
 def test_many_sequences(gpu):
     """More than a search step's 64 and than 64 * 64, empty ones among them."""
     rng = random.Random(3)
@@ -124,12 +149,10 @@ def test_many_sequences(gpu):
     t = sum(lengths)
     q = random_heads(g, t, 2, 16, torch.bfloat16, gpu)
     k, v = (random_heads(g, t, 1, 16, torch.bfloat16, gpu) for _ in range(2))
-    got = prompt_attention(q, k, v, starts_of(lengths, gpu))
+    got = check(q, k, v, lengths)
     assert torch.equal(got, prompt_attention(q, k, v, starts_of(lengths, gpu, torch.int64)))
-    short = [n for n in lengths[:150]]
-    s = sum(short)
-    assert torch.equal(got[:s], check(q[:s], k[:s], v[:s], short))
-    assert torch.equal(got[-70:], check(q[-70:], k[-70:], v[-70:], [70]))
+    for few in (lengths[:65], lengths[:150]):
+        check(q[:sum(few)], k[:sum(few)], v[:sum(few)], few)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -215,14 +238,19 @@ def test_strides(gpu):
     assert torch.equal(got, prompt_attention(q, one.repeat(1, 2, 1), v, starts_of(lengths, gpu)))
 
 
-def test_a_sequence_does_not_depend_on_its_neighbours(gpu):
+def test_neighbours_values_do_not_matter(gpu):
+    """The same bits beside other sequences' other values."""
     g = torch.Generator().manual_seed(61)
     lengths = [77, 300, 5]
-    q = random_heads(g, 382, 6, 128, torch.bfloat16, gpu)
-    k, v = (random_heads(g, 382, 3, 128, torch.bfloat16, gpu) for _ in range(2))
-    got = prompt_attention(q, k, v, starts_of(lengths, gpu))
-    alone = prompt_attention(*(t[77:377].contiguous() for t in (q, k, v)), starts_of([300], gpu))
-    assert torch.equal(got[77:377], alone)
+    for heads, kv in ((6, 3), (64, 32)):
+        q = random_heads(g, 382, heads, 128, torch.bfloat16, gpu)
+        k, v = (random_heads(g, 382, kv, 128, torch.bfloat16, gpu) for _ in range(2))
+        got = prompt_attention(q, k, v, starts_of(lengths, gpu))
+        for t in (q, k, v):
+            t[:77] *= 3
+            t[377:] = float("nan")
+        again = prompt_attention(q, k, v, starts_of(lengths, gpu))
+        assert torch.equal(got[77:377], again[77:377])
 
 
 def test_no_tokens_and_refusals(gpu):
