@@ -133,7 +133,7 @@ def test_every_form(gpu, dtype, dim, lengths, before, heads, kv, rows, split):
     k, v = (random_heads(g, sum(key_lengths), kv, dim, dtype, gpu) for _ in range(2))
     check(q, k, v, lengths, key_lengths)
     # rows behind the last sequence, and a sequence whose queries see nothing
-    few = [lengths[0], *lengths[1:-1], lengths[-1] - 2] if lengths[-1] > 2 else lengths
+    few = [*lengths[:-1], lengths[-1] - 2]
     got = check(q, k, v, few, key_lengths)
     assert (got[sum(few):] == 0).all()
     out = torch.full_like(q, 7.0)
