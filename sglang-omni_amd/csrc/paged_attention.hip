@@ -41,12 +41,22 @@ struct PagedParams {
 
 constexpr int kKeys = 32;  // of a tile
 constexpr int kWaves = 4;
+constexpr float kLazy = 6.f;
 constexpr int kLeastChunk = OMNI_PAGED_LEAST_CHUNK, kMostChunk = OMNI_PAGED_MOST_CHUNK;
 
-// The keys of a chunk: the least of 256, 512 and 1024 that leaves a sequence at most 32 chunks, or 1024.
-// Short chunks spread one stream over the chip; long ones write fewer parts.
-OMNI_DEVICE int chunk_of(int64_t length) {
-  return length <= 32 * kLeastChunk ? kLeastChunk : length <= 64 * kLeastChunk ? 2 * kLeastChunk : kMostChunk;
+// The keys of a chunk. Short chunks spread one stream over the chip, long ones have fewer starts and parts:
+// with 256, 512 and 1024 for all lengths 1 x 2000 took 13.4, 16.8 and 25.2 us, 1 x 9000 23.4, 23.7 and 30.9,
+// 64 up to 5000 174, 160 and 158, 2 x 131072 176, 175 and 170 (E4M3).
+OMNI_DEVICE int chunk_of(int length) {
+  return length <= 8 * kLeastChunk ? kLeastChunk : length <= 64 * kLeastChunk ? 2 * kLeastChunk : kMostChunk;
+}
+
+// The keys that sequence b's query sees: within the table's room and max_length.
+OMNI_DEVICE int length_of(const PagedParams& p, int b) {
+  const int64_t given = p.wide ? static_cast<const int64_t*>(p.lengths)[b]
+                               : (int64_t) static_cast<const int32_t*>(p.lengths)[b];
+  const int64_t room = p.columns * p.cache.page_size, most = room < p.max_length ? room : p.max_length;
+  return (int)(given < 0 ? 0 : given > most ? most : given);
 }
 
 // Eight E4M3 bytes as bf16 or float16, exactly.
@@ -98,7 +108,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
   // keys' rows (element offsets, negative: left out), their scales, V tiles of the waves; at the end
   // the waves' outputs
   __shared__ int64_t rows[kMostChunk];
-  __shared__ float scales[kBytes ? 2 : 1][kBytes ? kMostChunk : 1];
+  __shared__ __attribute__((aligned(16))) float scales[kBytes ? 2 : 1][kBytes ? kMostChunk : 4];
   __shared__ __attribute__((aligned(16))) uint8_t tiles[kWaves][kKeys * D * 2];
   __shared__ float stats[kWaves][2][16];
 
@@ -107,26 +117,23 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
   const int chunk = blockIdx.x;
   const int kv_head = blockIdx.y / p.head_tiles, head_tile = blockIdx.y % p.head_tiles;
   const int b = blockIdx.z;
-  const int64_t given = p.wide ? static_cast<const int64_t*>(p.lengths)[b]
-                               : (int64_t) static_cast<const int32_t*>(p.lengths)[b];
-  const int64_t room = p.columns * p.cache.page_size;
-  const int64_t most = room < p.max_length ? room : p.max_length;
-  const int length = (int)(given < 0 ? 0 : given > most ? most : given);
+  const int length = length_of(p, b);
   const int size = chunk_of(length);
   const int chunks = (length + size - 1) / size;
   if (chunk > 0 && chunk >= chunks) return;
   const int first = chunk * size, count = length - first < size ? length - first : size;
 
-  for (int i = threadIdx.x; i < count; i += 64 * kWaves) {
+  // the rows of whole tiles: one past the chunk is left out, as on a page outside the cache
+  for (int i = threadIdx.x; i < (count + kKeys - 1) / kKeys * kKeys; i += 64 * kWaves) {
     const uint32_t key = (uint32_t)(first + i), column_of = key / (uint32_t)p.cache.page_size;
-    const int page = p.table[b * p.table_row + column_of];
+    const int page = i < count ? p.table[b * p.table_row + column_of] : -1;
     const uint32_t offset = key - column_of * (uint32_t)p.cache.page_size;
     const bool held = page >= 0 && page < p.cache.pages;
     rows[i] = held ? page * p.cache.page + offset * p.cache.token + kv_head * p.cache.head : -1;
     if constexpr (kBytes) {
       const int64_t at = (int64_t)page * p.cache.scale_page + offset * p.cache.scale_token +
                          kv_head * p.cache.scale_head;
-      scales[0][i] = held ? p.cache.key_scale[at] : 0.f;
+      scales[0][i] = held ? p.cache.key_scale[at] * p.scale : 0.f;
       scales[1][i] = held ? p.cache.value_scale[at] : 0.f;
     }
   }
@@ -150,33 +157,54 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
   f32x4 o[D / 16];
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -__builtin_inff(), l = 0.f;
+  float m = -__builtin_inff(), m_use = 0.f, l = 0.f;
   __syncthreads();
 
+  // A tile's rows in registers: loads without branches, so that all are on their way at once. Rows that are
+  // left out read the cache's first one.
+  u32x4 k[2][kLoads], v[kVLoads];
+  const int64_t spare = kv_head * p.cache.head;
   const u32x4 nothing = {0u, 0u, 0u, 0u};
-  for (int at = wave * kKeys; at < count; at += kWaves * kKeys) {
-    u32x4 k[2][kLoads], v[kVLoads];
+  bool k_whole;  // no row of this lane is left out
+  auto load_keys = [&](int at) __attribute__((always_inline)) {
+    k_whole = true;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int i = at + t * 16 + column;
-      const int64_t row = i < count ? rows[i] : -1;
+      const int64_t row = rows[at + t * 16 + column];
+      k_whole &= row >= 0;
+      const uint8_t* from = p.cache.keys + (row >= 0 ? row : spare) * sizeof(H);
 #pragma unroll
       for (int s = 0; s < kLoads; ++s) {
         const int byte = s * 64 + quarter * 16;
-        k[t][s] = nothing;
-        if (row >= 0 && byte < p.dim * (int)sizeof(H))
-          k[t][s] = *reinterpret_cast<const u32x4*>(p.cache.keys + row * sizeof(H) + byte);
+        k[t][s] = *reinterpret_cast<const u32x4*>(from + (byte < p.dim * (int)sizeof(H) ? byte : 0));
       }
     }
+  };
+  auto load_values_of = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < kVLoads; ++s) {
-      const int piece = s * 64 + lane, r = piece / (kRow / 16), byte = piece % (kRow / 16) * 16;
-      const int64_t row = at + r < count ? rows[at + r] : -1;
-      v[s] = nothing;
-      if (row >= 0 && byte < p.dim * (int)sizeof(H))
-        v[s] = *reinterpret_cast<const u32x4*>(p.cache.values + row * sizeof(H) + byte);
+      const int piece = s * 64 + lane, byte = piece % (kRow / 16) * 16;
+      const int64_t row = rows[at + piece / (kRow / 16)];
+      v[s] = *reinterpret_cast<const u32x4*>(p.cache.values + (row >= 0 ? row : spare) * sizeof(H) +
+                                             (byte < p.dim * (int)sizeof(H) ? byte : 0));
     }
-
+  };
+  uint8_t* const tile = tiles[wave];
+  int at = wave * kKeys;
+  if (at < count) {
+    load_keys(at);
+    load_values_of(at);
+  }
+  for (; at < count; at += kWaves * kKeys) {
+    const bool whole = __ballot(!k_whole) == 0;  // the same rows for keys and values
+    const int next = at + kWaves * kKeys;
+    if (p.dim < D) {  // q is zero behind the head, and so must be what it meets
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int s = 0; s < kLoads; ++s)
+          if (s * 64 + quarter * 16 >= p.dim * (int)sizeof(H)) k[t][s] = nothing;
+    }
     f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -191,8 +219,13 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
         s[t] = O::mfma16(a, q[c], s[t]);
       }
     }
+    if (next < count) load_keys(next);
+    if (!whole) {  // what a row left out holds must not meet a weight of zero
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i)
+        if (rows[at + (i * 64 + lane) / (kRow / 16)] < 0) v[i] = nothing;
+    }
     // V to shared memory as it will be read
-    uint8_t* tile = tiles[wave];
 #pragma unroll
     for (int i = 0; i < kVLoads; ++i) {
       const int piece = i * 64 + lane, r = piece / (kRow / 16), at16 = piece % (kRow / 16);
@@ -204,38 +237,46 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
         *reinterpret_cast<u32x4*>(tile + (r * kPieces + v_slot<D>(r, at16)) * 16) = v[i];
       }
     }
+    if (next < count) load_values_of(next);
 
     // lane (column, quarter) holds keys 16 t + 4 quarter .. + 3 of head `column`
-    float weight_scale[2][4];
+    f32x4 value_scale[2];
     float top = -__builtin_inff();
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = at + t * 16 + quarter * 4 + e;
-        const bool seen = i < count && rows[i] >= 0;
-        if constexpr (kBytes) {
-          s[t][e] *= seen ? scales[0][i] : 0.f;
-          weight_scale[t][e] = seen ? scales[1][i] : 0.f;
-        }
-        s[t][e] = seen ? s[t][e] * p.scale : -__builtin_inff();
-        top = fmaxf(top, s[t][e]);
+    for (int t = 0; t < 2; ++t) {
+      const int i = at + t * 16 + quarter * 4;
+      if constexpr (kBytes) {
+        s[t] *= *reinterpret_cast<const f32x4*>(&scales[0][i]);
+        value_scale[t] = *reinterpret_cast<const f32x4*>(&scales[1][i]);
+      } else {
+        s[t] *= p.scale;
       }
-    const float m_new = fmaxf(m, column_max(top));
-    const float m_use = m_new == -__builtin_inff() ? 0.f : m_new;
-    const float keep = __builtin_amdgcn_exp2f(m - m_use);
-    m = m_new;
-    l *= keep;
+      if (!whole) {
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) o[d] *= keep;
+        for (int e = 0; e < 4; ++e) s[t][e] = rows[i + e] >= 0 ? s[t][e] : -__builtin_inff();
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[t][e]);
+    }
+    // the maximum moves only where a score is past it by more than 2^kLazy, as in the prompt kernel
+    if (__ballot(top > m + kLazy) != 0) {
+      const float m_new = fmaxf(m, column_max(top));
+      m_use = m_new == -__builtin_inff() ? 0.f : m_new;
+      const float keep = __builtin_amdgcn_exp2f(m - m_use);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[d] *= keep;
+    }
+    const float shift = P::kBias - m_use;
     typename P::x8 w, w_low;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float x = __builtin_amdgcn_exp2f(s[t][e] - m_use + P::kBias);
+        float x = __builtin_amdgcn_exp2f(s[t][e] + shift);
         l += x;
-        if constexpr (kBytes) x *= weight_scale[t][e];
+        if constexpr (kBytes) x *= value_scale[t][e];
         w[t * 4 + e] = (PT)x;
         w_low[t * 4 + e] = (PT)(x - (float)w[t * 4 + e]);
       }
@@ -263,12 +304,12 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
   float m_all = stats[0][0][column];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, stats[w][0][column]);
-  const float m_use = m_all == -__builtin_inff() ? 0.f : m_all;
+  const float m_base = m_all == -__builtin_inff() ? 0.f : m_all;
   float l_all = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w)
-    l_all += stats[w][1][column] * __builtin_amdgcn_exp2f(stats[w][0][column] - m_use);
-  const float keep = __builtin_amdgcn_exp2f(m - m_use);
+    l_all += stats[w][1][column] * __builtin_amdgcn_exp2f(stats[w][0][column] - m_base);
+  const float keep = __builtin_amdgcn_exp2f(m - m_base);
   // [16 heads][D + 4] of a wave at a time
   constexpr int kPitch = D + 4;
   static_assert(sizeof(tiles) >= 16 * kPitch * 4, "a wave's outputs fit the tiles");
@@ -314,33 +355,50 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
   }
 }
 
-// The chunks of a (sequence, head) joined in their order: a workgroup, a thread to a dimension.
+// The chunks of a (sequence, head) joined: a workgroup of 4 waves, a quarter-wave to a row of up to 64
+// dimensions (4 a lane), so 16 chunks at a time, their sums joined in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
   const int heads = p.kv_heads * p.group;
   const int b = blockIdx.x / heads, head = blockIdx.x % heads;
-  const int64_t given = p.wide ? static_cast<const int64_t*>(p.lengths)[b]
-                               : (int64_t) static_cast<const int32_t*>(p.lengths)[b];
-  const int64_t room = p.columns * p.cache.page_size;
-  const int64_t most = room < p.max_length ? room : p.max_length;
-  const int length = (int)(given < 0 ? 0 : given > most ? most : given);
+  const int length = length_of(p, b);
   const int size = chunk_of(length), chunks = (length + size - 1) / size;
   if (chunks <= 1) return;
   const int64_t at = ((int64_t)b * heads + head) * p.chunks;
   const float* stats = p.parts + (int64_t)p.batch * heads * p.chunks * p.dim + at * 2;
+  __shared__ float sums[16][64 + 1][4];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 4, quad = threadIdx.x & 15;
   float m = -__builtin_inff();
-  for (int c = 0; c < chunks; ++c) m = fmaxf(m, stats[2 * c]);
+  for (int c = lane; c < chunks; c += 64) m = fmaxf(m, stats[2 * c]);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
   const float m_use = m == -__builtin_inff() ? 0.f : m;
-  for (int d = threadIdx.x; d < p.dim; d += blockDim.x) {
-    float l = 0.f, o = 0.f;
-    for (int c = 0; c < chunks; ++c) {
-      const float keep = __builtin_amdgcn_exp2f(stats[2 * c] - m_use);
-      l = __builtin_fmaf(stats[2 * c + 1], keep, l);
-      o = __builtin_fmaf(p.parts[(at + c) * p.dim + d], keep, o);
-    }
-    reinterpret_cast<T*>(p.out + b * p.out_row + head * p.out_head)[d] =
-        (T)(m == -__builtin_inff() ? 0.f : o / l);
+  float l = 0.f;
+  f32x4 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c = part; c < chunks; c += 16) {
+    const float keep = __builtin_amdgcn_exp2f(stats[2 * c] - m_use);
+    l = __builtin_fmaf(stats[2 * c + 1], keep, l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i * 64 + quad * 4 < p.dim)
+        o[i] += *reinterpret_cast<const f32x4*>(p.parts + (at + c) * p.dim + i * 64 + quad * 4) * keep;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(sums[part][i * 16 + quad]) = o[i];
+  if (quad == 0) sums[part][64][0] = l;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= p.dim) return;
+  float total = 0.f, l_all = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    total += sums[i][d / 4][d % 4];
+    l_all += sums[i][64][0];
+  }
+  reinterpret_cast<T*>(p.out + b * p.out_row + head * p.out_head)[d] =
+      (T)(m == -__builtin_inff() ? 0.f : total / l_all);
 }
 
 template <typename T, typename H, int D>
@@ -350,8 +408,8 @@ int launch_paged(const PagedParams& p, hipStream_t stream) {
                      dim3(64 * kWaves), 0, stream, p);
   OMNI_LAUNCH_CHECK();
   if (p.chunks > 1) {
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(p.batch * p.kv_heads * p.group)), dim3(D < 128 ? 64 : 128),
-                       0, stream, p);
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(p.batch * p.kv_heads * p.group)), dim3(256), 0,
+                       stream, p);
     OMNI_LAUNCH_CHECK();
   }
   return OMNI_OK;
@@ -388,10 +446,12 @@ extern "C" int omni_paged_attention(const omni_paged_args* a, omni_stream_t stre
   const int64_t kv_heads = a->cache->kv_heads, group = a->heads / kv_heads;
   const int64_t tiles = (group + 15) / 16;
   if (kv_heads * tiles > 65535 || a->batch * a->heads > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
-  // the most chunks of a length up to max_length: 32 up to 16384 keys, then one for each 1024
-  const int64_t few = (a->max_length + kLeastChunk - 1) / kLeastChunk;
-  const int64_t many = (a->max_length + kMostChunk - 1) / kMostChunk;
-  const int64_t chunks = few < 32 ? (few > 0 ? few : 1) : many > 32 ? many : 32;
+  // the most chunks of a length up to max_length: at most 8 up to 2048, then 32 up to 16384
+  auto pieces = [&](int64_t size) { return (a->max_length + size - 1) / size; };
+  int64_t chunks = pieces(kLeastChunk);
+  if (chunks > 8) chunks = pieces(2 * kLeastChunk) > 8 ? pieces(2 * kLeastChunk) : 8;
+  if (chunks > 32) chunks = pieces(kMostChunk) > 32 ? pieces(kMostChunk) : 32;
+  if (chunks < 1) chunks = 1;
   if (chunks > 1 && (!a->workspace || !aligned_to(a->workspace, 16) ||
                      a->workspace_bytes < a->batch * a->heads * chunks * (a->cache->dim + 2) * 4))
     return OMNI_ERR_INVALID_ARG;

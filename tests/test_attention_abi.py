@@ -37,14 +37,14 @@ def test_constants_match_the_header():
 def _chunks(length):
     """The chunks of a sequence, by the kernel's rule."""
     least, most = N.PAGED_LEAST_CHUNK, N.PAGED_MOST_CHUNK
-    size = least if length <= 32 * least else 2 * least if length <= 64 * least else most
+    size = least if length <= 8 * least else 2 * least if length <= 64 * least else most
     return -(-length // size)
 
 
 def test_workspace_holds_the_parts_of_every_length():
-    for bound in [0, 1, 255, 256, 257, 8191, 8192, 8193, 16384, 16385, 32768, 32769, 40000, 131072]:
+    for bound in [0, 1, 255, 256, 257, 2048, 2049, 4096, 8191, 8192, 8193, 16384, 16385, 32768, 32769, 40000, 131072]:
         held = attention._workspace_bytes(3, 16, bound) // (3 * 18 * 4)
-        for length in {0, 1, 256, 257, 8192, 8193, 16384, 16385, bound}:
+        for length in {0, 1, 256, 257, 2048, 2049, 8192, 8193, 16384, 16385, bound}:
             if length <= bound:
                 assert _chunks(length) <= max(held, 1), (bound, length)
 

@@ -104,9 +104,9 @@ def test_lengths_around_every_edge(gpu, dtype, bytes_held, heads, kv, dim, page)
 
 @pytest.mark.parametrize("bytes_held", [False, True])
 def test_long_sequences(gpu, bytes_held):
-    """Chunks of every size: 8192 and 16384 are the last lengths of 256 and 512."""
+    """Chunks of every size: 2048 and 16384 are the last lengths of 256 and 512."""
     g = torch.Generator().manual_seed(5)
-    lengths = [8191, 8192, 8193, 16384, 16385, 40001, 2]
+    lengths = [2047, 2048, 2049, 16384, 16385, 40001, 2]
     pages = sum(-(-n // 64) for n in lengths)
     cache = filled_cache(g, pages, 64, 2, 64, E4M3 if bytes_held else torch.bfloat16, gpu)
     q = queries(g, len(lengths), 6, 64, torch.bfloat16, gpu, 4.0)
