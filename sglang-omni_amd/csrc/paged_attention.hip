@@ -294,64 +294,53 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
     }
   }
 
-  // the waves' parts joined, in their order
+  // The waves' parts joined: each leaves its heads' outputs in its tile's place, and a thread takes 4
+  // dimensions of a head from all of them, in their order.
   l = column_sum(l);
   if (quarter == 0) {
     stats[wave][0][column] = m;
     stats[wave][1][column] = l;
   }
-  __syncthreads();  // and every wave has read its last tile
-  float m_all = stats[0][0][column];
+  static_assert(sizeof(tiles[0]) >= 16 * D * 4, "a wave's outputs fit its tile");
+  auto place_of = [](int h, int quad) { return h * D + (quad ^ (h & 15)) * 4; };
+  const int heads_here = p.group - head_tile * 16 < 16 ? p.group - head_tile * 16 : 16;
+  if (column < heads_here) {
+    float* mine = reinterpret_cast<float*>(tile);
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, stats[w][0][column]);
-  const float m_base = m_all == -__builtin_inff() ? 0.f : m_all;
-  float l_all = 0.f;
+    for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(mine + place_of(column, d * 4 + quarter)) = o[d];
+  }
+  __syncthreads();
+  for (int item = threadIdx.x; item < heads_here * (D / 4); item += 64 * kWaves) {
+    const int h = item / (D / 4), quad = item % (D / 4), d = quad * 4;
+    if (d >= p.dim) continue;
+    float m_all = stats[0][0][h];
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    l_all += stats[w][1][column] * __builtin_amdgcn_exp2f(stats[w][0][column] - m_base);
-  const float keep = __builtin_amdgcn_exp2f(m - m_base);
-  // [16 heads][D + 4] of a wave at a time
-  constexpr int kPitch = D + 4;
-  static_assert(sizeof(tiles) >= 16 * kPitch * 4, "a wave's outputs fit the tiles");
-  float* sum = reinterpret_cast<float*>(tiles);
-  for (int turn = 0; turn < kWaves; ++turn) {
-    if (wave == turn) {
+    for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, stats[w][0][h]);
+    const float m_base = m_all == -__builtin_inff() ? 0.f : m_all;
+    float l_all = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        float* to = sum + column * kPitch + d * 16 + quarter * 4;
-        f32x4 x = o[d] * keep;
-        if (turn > 0) x += *reinterpret_cast<f32x4*>(to);
-        *reinterpret_cast<f32x4*>(to) = x;
+    for (int w = 0; w < kWaves; ++w) {
+      const float keep = __builtin_amdgcn_exp2f(stats[w][0][h] - m_base);
+      l_all = __builtin_fmaf(stats[w][1][h], keep, l_all);
+      x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(tiles[w]) + place_of(h, quad)) * keep;
+    }
+    const int out_head = kv_head * p.group + head_tile * 16 + h;
+    if (chunks > 1) {
+      const int64_t at = ((int64_t)b * p.kv_heads * p.group + out_head) * p.chunks + chunk;
+      *reinterpret_cast<f32x4*>(p.parts + at * p.dim + d) = x;
+      if (quad == 0) {
+        float* to = p.parts + (int64_t)p.batch * p.kv_heads * p.group * p.chunks * p.dim + at * 2;
+        to[0] = m_all;
+        to[1] = l_all;
       }
-    }
-    __syncthreads();
-  }
-  // 16 heads' rows out: 16 threads to a head
-  const int h = threadIdx.x >> 4, part = threadIdx.x & 15;
-  const int out_in_group = head_tile * 16 + h;
-  if (out_in_group >= p.group) return;
-  const int out_head = kv_head * p.group + out_in_group;
-  // the statistics of head h: lane h's (any quarter's) of this wave
-  const float m_h = __shfl(m_all, h), l_h = __shfl(l_all, h);
-  if (chunks > 1) {
-    const int64_t at = ((int64_t)b * p.kv_heads * p.group + out_head) * p.chunks + chunk;
-    for (int d = part * 4; d < p.dim; d += 64)
-      *reinterpret_cast<f32x4*>(p.parts + at * p.dim + d) = *reinterpret_cast<f32x4*>(sum + h * kPitch + d);
-    if (part == 0) {
-      float* to = p.parts + (int64_t)p.batch * p.kv_heads * p.group * p.chunks * p.dim + at * 2;
-      to[0] = m_h;
-      to[1] = l_h;
-    }
-    return;
-  }
-  const float unit = m_h == -__builtin_inff() ? 0.f : 1.f / l_h;
-  T* to = reinterpret_cast<T*>(p.out + b * p.out_row + out_head * p.out_head);
-  for (int d = part * 4; d < p.dim; d += 64) {
-    const f32x4 x = *reinterpret_cast<f32x4*>(sum + h * kPitch + d);
-    typename O::x4 y;
+    } else {
+      const float unit = m_all == -__builtin_inff() ? 0.f : 1.f / l_all;
+      typename O::x4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * unit);
-    *reinterpret_cast<typename O::x4*>(to + d) = y;
+      for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * unit);
+      *reinterpret_cast<typename O::x4*>(p.out + b * p.out_row + out_head * p.out_head + d * 2) = y;
+    }
   }
 }
 
