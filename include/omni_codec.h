@@ -1062,7 +1062,7 @@ int omni_prompt_attention(const omni_prompt_args* args, omni_stream_t stream);
  * multiple of 16 up to 256; batch up to 65535; scale positive. workspace: with L = OMNI_PAGED_LEAST_CHUNK
  * and c = ceil(max_length / L) up to 8, else max(8, ceil(max_length / 2 L)) up to 32, else max(32,
  * ceil(max_length / OMNI_PAGED_MOST_CHUNK)), at least batch * heads * c * (dim + 2) * 4 bytes, 16-byte
- * aligned; none for c up to 1. batch = 0 does nothing.
+ * aligned; none for a max_length up to 2 L. batch = 0 does nothing.
  */
 enum { OMNI_PAGED_LEAST_CHUNK = 256, OMNI_PAGED_MOST_CHUNK = 1024 };
 typedef struct omni_paged_args {

@@ -46,9 +46,13 @@ constexpr int kLeastChunk = OMNI_PAGED_LEAST_CHUNK, kMostChunk = OMNI_PAGED_MOST
 
 // The keys of a chunk. Short chunks spread one stream over the chip, long ones have fewer starts and parts:
 // with 256, 512 and 1024 for all lengths 1 x 2000 took 13.4, 16.8 and 25.2 us, 1 x 9000 23.4, 23.7 and 30.9,
-// 64 up to 5000 174, 160 and 158, 2 x 131072 176, 175 and 170 (E4M3).
+// 64 up to 5000 174, 160 and 158, 2 x 131072 176, 175 and 170 (E4M3). Up to 512 keys are one chunk, which
+// needs no second launch.
 OMNI_DEVICE int chunk_of(int length) {
-  return length <= 8 * kLeastChunk ? kLeastChunk : length <= 64 * kLeastChunk ? 2 * kLeastChunk : kMostChunk;
+  return length <= 2 * kLeastChunk    ? 2 * kLeastChunk
+         : length <= 8 * kLeastChunk  ? kLeastChunk
+         : length <= 64 * kLeastChunk ? 2 * kLeastChunk
+                                      : kMostChunk;
 }
 
 // The keys that sequence b's query sees: within the table's room and max_length.
@@ -180,13 +184,16 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
       }
     }
   };
+  // The values past the caches: nothing reads them again. (A line of keys is read in two halves.) 2 x 131072
+  // in 8 bits 127 -> 108 us, 128 x 1000 115 -> 93; the keys so too 122 and 110.
   auto load_values_of = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < kVLoads; ++s) {
       const int piece = s * 64 + lane, byte = piece % (kRow / 16) * 16;
       const int64_t row = rows[at + piece / (kRow / 16)];
-      v[s] = *reinterpret_cast<const u32x4*>(p.cache.values + (row >= 0 ? row : spare) * sizeof(H) +
-                                             (byte < p.dim * (int)sizeof(H) ? byte : 0));
+      v[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(
+          p.cache.values + (row >= 0 ? row : spare) * sizeof(H) +
+          (byte < p.dim * (int)sizeof(H) ? byte : 0)));
     }
   };
   uint8_t* const tile = tiles[wave];
@@ -435,12 +442,12 @@ extern "C" int omni_paged_attention(const omni_paged_args* a, omni_stream_t stre
   const int64_t kv_heads = a->cache->kv_heads, group = a->heads / kv_heads;
   const int64_t tiles = (group + 15) / 16;
   if (kv_heads * tiles > 65535 || a->batch * a->heads > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
-  // the most chunks of a length up to max_length: at most 8 up to 2048, then 32 up to 16384
+  // the most chunks of a length up to max_length: one up to 512, at most 8 up to 2048, then 32 up to 16384
   auto pieces = [&](int64_t size) { return (a->max_length + size - 1) / size; };
   int64_t chunks = pieces(kLeastChunk);
   if (chunks > 8) chunks = pieces(2 * kLeastChunk) > 8 ? pieces(2 * kLeastChunk) : 8;
   if (chunks > 32) chunks = pieces(kMostChunk) > 32 ? pieces(kMostChunk) : 32;
-  if (chunks < 1) chunks = 1;
+  if (a->max_length <= 2 * kLeastChunk) chunks = 1;
   if (chunks > 1 && (!a->workspace || !aligned_to(a->workspace, 16) ||
                      a->workspace_bytes < a->batch * a->heads * chunks * (a->cache->dim + 2) * 4))
     return OMNI_ERR_INVALID_ARG;

@@ -108,12 +108,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
 
 def _workspace_bytes(rows: int, dim: int, max_length: int) -> int:
     """What omni_paged_attention needs for the parts of `rows` heads of all sequences."""
+    if max_length <= 2 * N.PAGED_LEAST_CHUNK:
+        return 0
     chunks = -(-max_length // N.PAGED_LEAST_CHUNK)
     if chunks > 8:
         chunks = max(8, -(-max_length // (2 * N.PAGED_LEAST_CHUNK)))
         if chunks > 32:
             chunks = max(32, -(-max_length // N.PAGED_MOST_CHUNK))
-    return rows * chunks * (dim + 2) * 4 if chunks > 1 else 0
+    return rows * chunks * (dim + 2) * 4
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKvCache, table: torch.Tensor, lengths: torch.Tensor,

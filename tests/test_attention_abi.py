@@ -37,14 +37,16 @@ def test_constants_match_the_header():
 def _chunks(length):
     """The chunks of a sequence, by the kernel's rule."""
     least, most = N.PAGED_LEAST_CHUNK, N.PAGED_MOST_CHUNK
+    if length <= 2 * least:
+        return 1
     size = least if length <= 8 * least else 2 * least if length <= 64 * least else most
     return -(-length // size)
 
 
 def test_workspace_holds_the_parts_of_every_length():
-    for bound in [0, 1, 255, 256, 257, 2048, 2049, 4096, 8191, 8192, 8193, 16384, 16385, 32768, 32769, 40000, 131072]:
+    for bound in [0, 1, 255, 256, 257, 512, 513, 2048, 2049, 4096, 8191, 8192, 8193, 16384, 16385, 32768, 32769, 40000, 131072]:
         held = attention._workspace_bytes(3, 16, bound) // (3 * 18 * 4)
-        for length in {0, 1, 256, 257, 2048, 2049, 8192, 8193, 16384, 16385, bound}:
+        for length in {0, 1, 256, 257, 512, 513, 2048, 2049, 8192, 8193, 16384, 16385, bound}:
             if length <= bound:
                 assert _chunks(length) <= max(held, 1), (bound, length)
 
@@ -104,8 +106,8 @@ def test_refused_before_any_launch():
     for kw in ({"cache": 0}, {"dtype": N.DTYPE_F32}, {"scale": 0.0}, {"q_stride_head": 12},
                {"lengths_dtype": N.DTYPE_F32}, {"max_length": -1}, {"batch": -1}, {"batch": 2, "q": 0},
                {"batch": 2, "lengths": 4098}, {"batch": 2, "table": 0},
-               {"batch": 2, "max_length": 257}, {"batch": 2, "max_length": 257, "workspace": 4096,
-                                                 "workspace_bytes": 2 * 4 * 2 * 18 * 4 - 1}):
+               {"batch": 2, "max_length": 513}, {"batch": 2, "max_length": 513, "workspace": 4096,
+                                                 "workspace_bytes": 2 * 4 * 3 * 18 * 4 - 1}):
         assert paged_status(**kw) == N.INVALID_ARG, kw
     assert paged_status(batch=65536) == paged_status(max_length=2**31 - 1) == N.UNSUPPORTED
 
