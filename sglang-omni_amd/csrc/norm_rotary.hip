@@ -76,7 +76,11 @@ OMNI_DEVICE void store_bytes(uint8_t* dst, int valid, const float (&v)[V], float
 // chunks of two runs of V values: in the half layout V pairs' first and second values, interleaved V /
 // 2 pairs of the first half of the pairs and as many of the second; of what is not turned one run of
 // each half (in turn where it has no halves). A chunk's sines and cosines serve all HP heads.
-template <typename T, int V, int ITERS, int HP>
+//
+// WHOLE: every run of a chunk lies in the head. Then a lane's loads, of rows, weights, position and
+// frequencies, have no branch around them and go out at once (a load under a branch is waited for before
+// the next one goes out); lanes past the last chunk load it too and count nothing.
+template <typename T, int V, int ITERS, int HP, bool WHOLE>
 __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
   const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> p.lane_shift;
   if (item >= p.items) return;
@@ -104,13 +108,16 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
   const bool single = V == 1 && p.interleaved;
 #pragma unroll
   for (int t = 0; t < ITERS; ++t) {
-    const int chunk = lane + t * lanes, copied = chunk - p.turned_chunks;
+    const int mine = lane + t * lanes, chunk = WHOLE && mine >= p.chunks ? p.chunks - 1 : mine;
+    const int copied = chunk - p.turned_chunks;
     const bool turned = chunk < p.turned_chunks;
     at0[t] = turned ? chunk * (single ? 2 : V) : past + copied * (halves ? V : 2 * V);
     at1[t] = turned ? (single ? at0[t] + 1 : at0[t] + p.pairs) : at0[t] + (halves ? rest / 2 : V);
-    valid0[t] = chunk < p.chunks ? p.dim - at0[t] : 0;
-    valid1[t] = chunk < p.chunks ? p.dim - at1[t] : 0;
+    valid0[t] = mine < p.chunks ? p.dim - at0[t] : 0;
+    valid1[t] = mine < p.chunks ? p.dim - at1[t] : 0;
   }
+  double position = 0.0;
+  if (p.pairs > 0) position = (double)load_index(p.positions, p.positions64, token * p.position_stride);
 
   float a[HP][ITERS][V], b[HP][ITERS][V];
 #pragma unroll
@@ -118,8 +125,8 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
     const T* row = src + (head0 + i < heads ? head0 + i : heads - 1) * src_head;
 #pragma unroll
     for (int t = 0; t < ITERS; ++t) {
-      load_values(row + at0[t], valid0[t], a[i][t]);
-      load_values(row + at1[t], valid1[t], b[i][t]);
+      load_values(row + at0[t], WHOLE ? V : valid0[t], a[i][t]);
+      load_values(row + at1[t], WHOLE ? V : valid1[t], b[i][t]);
     }
   }
   if (p.normed && kind < 2) {
@@ -128,8 +135,8 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
 #pragma unroll
     for (int t = 0; t < ITERS; ++t) {
       if (weight) {
-        load_values(weight + at0[t], valid0[t], w0[t]);
-        load_values(weight + at1[t], valid1[t], w1[t]);
+        load_values(weight + at0[t], WHOLE ? V : valid0[t], w0[t]);
+        load_values(weight + at1[t], WHOLE ? V : valid1[t], w1[t]);
       } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) w0[t][v] = w1[t][v] = 1.f;
@@ -139,10 +146,13 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
     for (int i = 0; i < HP; ++i) {
       float sum = 0.f;
 #pragma unroll
-      for (int t = 0; t < ITERS; ++t)
+      for (int t = 0; t < ITERS; ++t) {
+        float part = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v)
-          sum = __builtin_fmaf(a[i][t][v], a[i][t][v], __builtin_fmaf(b[i][t][v], b[i][t][v], sum));
+          part = __builtin_fmaf(a[i][t][v], a[i][t][v], __builtin_fmaf(b[i][t][v], b[i][t][v], part));
+        sum += WHOLE && valid0[t] == 0 ? 0.f : part;
+      }
       for (int off = 1; off < lanes; off <<= 1) sum += __shfl_xor(sum, off);
       const float r = 1.f / sqrtf(sum / (float)p.dim + p.eps);
 #pragma unroll
@@ -155,7 +165,6 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
     }
   }
   if (p.pairs > 0 && kind < 2) {
-    const double position = (double)load_index(p.positions, p.positions64, token * p.position_stride);
 #pragma unroll
     for (int t = 0; t < ITERS; ++t) {
       const int chunk = lane + t * lanes;
@@ -209,8 +218,9 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
         if (head0 + i >= heads) break;
 #pragma unroll
         for (int t = 0; t < ITERS; ++t) {
-          store_values(dst + (head0 + i) * dst_head + at0[t], valid0[t], a[i][t]);
-          store_values(dst + (head0 + i) * dst_head + at1[t], valid1[t], b[i][t]);
+          if (WHOLE && valid0[t] == 0) continue;
+          store_values(dst + (head0 + i) * dst_head + at0[t], WHOLE ? V : valid0[t], a[i][t]);
+          store_values(dst + (head0 + i) * dst_head + at1[t], WHOLE ? V : valid1[t], b[i][t]);
         }
       }
     }
@@ -249,6 +259,7 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
     }
 #pragma unroll
     for (int t = 0; t < ITERS; ++t) {
+      if (WHOLE && valid0[t] == 0) continue;
       if (p.held == OMNI_DTYPE_FP8_E4M3) {
         store_bytes(held + at + at0[t], valid0[t], a[i][t], unit);
         store_bytes(held + at + at1[t], valid1[t], b[i][t], unit);
@@ -263,13 +274,13 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
   }
 }
 
-template <typename T, int V, int ITERS, int HP>
+template <typename T, int V, int ITERS, int HP, bool WHOLE>
 int launch_heads(HeadsParams p, int64_t tokens, hipStream_t stream) {
   for (int kind = 0; kind < 3; ++kind) p.groups[kind] = (p.heads[kind] + HP - 1) / HP;
   p.items = tokens * (p.groups[0] + p.groups[1] + p.groups[2]);
   const int64_t workgroups = ((p.items << p.lane_shift) + 255) / 256;
   if (workgroups > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((heads_kernel<T, V, ITERS, HP>), dim3((unsigned)workgroups), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((heads_kernel<T, V, ITERS, HP, WHOLE>), dim3((unsigned)workgroups), dim3(256), 0, stream, p);
   OMNI_LAUNCH_CHECK();
   return OMNI_OK;
 }
@@ -282,8 +293,14 @@ int launch_chunks(HeadsParams p, int64_t tokens, hipStream_t stream) {
   p.chunks = p.turned_chunks + (p.dim - 2 * p.pairs + 2 * V - 1) / (2 * V);
   for (p.lane_shift = 0; (1 << p.lane_shift) * ITERS < p.chunks;) ++p.lane_shift;
   const int64_t lanes = (tokens * (p.heads[0] + p.heads[1] + p.heads[2]) / 4) << p.lane_shift;
-  return lanes >= 512 * 256 ? launch_heads<T, V, ITERS, 4>(p, tokens, stream)
-                            : launch_heads<T, V, ITERS, 1>(p, tokens, stream);
+  const bool many = lanes >= 512 * 256;
+  if constexpr (V > 1) {
+    if ((p.dim - 2 * p.pairs) % (2 * V) == 0)
+      return many ? launch_heads<T, V, ITERS, 4, true>(p, tokens, stream)
+                  : launch_heads<T, V, ITERS, 1, true>(p, tokens, stream);
+  }
+  return many ? launch_heads<T, V, ITERS, 4, false>(p, tokens, stream)
+              : launch_heads<T, V, ITERS, 1, false>(p, tokens, stream);
 }
 
 // V: the most of 8, 4, 1 that divide the pairs (or, where nothing is turned, half the head); a head of
