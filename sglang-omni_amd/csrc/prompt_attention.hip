@@ -64,7 +64,7 @@ OMNI_DEVICE int v_slot(int r, int p) {
 // way. Not LONG, for few rows: the waves share 32 rows and each owns every NW-th tile, [NW][K, V], and
 // their parts are joined at the end; so many more workgroups, each with fewer tiles one after the other.
 template <typename T, int D, int NW, bool LONG>
-__global__ void __launch_bounds__(64 * NW, D < 256 ? 2 : 1) prompt_kernel(const PromptParams p) {
+__global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) prompt_kernel(const PromptParams p) {
   using O = Op<T>;
   constexpr int kRows = LONG ? 32 * NW : 32;
   constexpr int kKeys = keys_of(D, LONG), kBlocks = kKeys / 32, kSteps = kKeys / 16;
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(64 * NW, D < 256 ? 2 : 1) prompt_kernel(const 
   // holds its own head's keys. The last tiles of a sequence, which see the most keys, go first.
   const int kv_head = blockIdx.x % p.kv_heads;
   const int split = blockIdx.x / p.kv_heads % p.splits;
-  const int slot = p.slots - 1 - blockIdx.x / p.kv_heads / p.splits;
+  const int slot = blockIdx.x / p.kv_heads / p.splits;
   // Sequence s owns the tiles from floor(first row / kRows) + s on: never fewer than it needs, and
   // found by search without a sum over the sequences before it: 64 at a time, each lane one's bounds.
   int lo = 0, n = p.sequences;
@@ -111,8 +111,9 @@ __global__ void __launch_bounds__(64 * NW, D < 256 ? 2 : 1) prompt_kernel(const 
     n = n - found * step < step ? n - found * step : step;
   }
   const int queries = last - first, rows = queries * p.group;
-  const int row0 = (slot - (first * p.group / kRows + lo)) * kRows;
-  if (queries <= 0 || row0 < 0 || row0 >= rows) return;
+  const int at_slot = slot - (first * p.group / kRows + lo), row_tiles = (rows + kRows - 1) / kRows;
+  if (queries <= 0 || at_slot < 0 || at_slot >= row_tiles) return;
+  const int row0 = (row_tiles - 1 - at_slot) * kRows;
   const int keys = key_last > key_first ? key_last - key_first : 0;
 
   // this lane's row, and how many keys it, the wave's first and last row and the tile's last see
@@ -441,15 +442,39 @@ __global__ void __launch_bounds__(64 * NW, D < 256 ? 2 : 1) prompt_kernel(const 
     return;
   }
 
-  if (wave_row + column >= rows) return;
   l = half_sum(l);
+  const bool stored = wave_row + column < rows;
+  if (p.splits > 1) {
+    if (!stored) return;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d * 32 + i * 8 + half * 4 < p.dim)
+          store_row(query, head, d * 32 + i * 8 + half * 4,
+                    f32x4{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]}, m, l);
+    return;
+  }
+  // A lane holds 4 dimensions of each 8; with the other half-wave's of one 8 for its own of the next it
+  // stores 16 bytes at a time.
+  const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
+  uint8_t* to = p.out + (int64_t)(first + query) * p.out_token + head * p.out_head;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (d * 32 + i * 8 + half * 4 < p.dim)
-        store_row(query, head, d * 32 + i * 8 + half * 4,
-                  f32x4{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]}, m, l);
+    for (int i = 0; i < 4; i += 2) {
+      typename O::x4 x, y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = (T)(o[d][i * 4 + j] * unit);
+        y[j] = (T)(o[d][i * 4 + 4 + j] * unit);
+      }
+      const u32x2 a = __builtin_bit_cast(u32x2, x), b = __builtin_bit_cast(u32x2, y);
+      const auto r0 = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+      const auto r1 = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+      const int at = d * 32 + (i + half) * 8;
+      if (stored && at < p.dim) *reinterpret_cast<u32x4*>(to + at * 2) = u32x4{r0[0], r1[0], r0[1], r1[1]};
+    }
 }
 
 // The parts of a row's keys joined in their order: 4 dimensions a thread. Rows of no sequence have no
