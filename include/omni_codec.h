@@ -1001,10 +1001,19 @@ int omni_norm_rotary(const omni_norm_rotary_args* args, omni_stream_t stream);
  * f16, f32), rounded once; a slot that is not in the cache gives zeros. dim a multiple of 16, rows of
  * the cache 16-byte aligned; k and v of any alignment of their type. tokens = 0 does nothing.
  */
-int omni_read_cache(const omni_kv_cache* cache, const void* slots, int slots_dtype,
-                    int64_t slots_stride, int64_t tokens, void* k, int64_t k_stride_token,
-                    int64_t k_stride_head, void* v, int64_t v_stride_token, int64_t v_stride_head,
-                    int dtype, omni_stream_t stream);
+typedef struct omni_read_cache_args {
+  const omni_kv_cache* cache;
+  const void* slots;
+  int slots_dtype;
+  int64_t slots_stride;
+  int64_t tokens;
+  void* k;
+  int64_t k_stride_token, k_stride_head;
+  void* v;
+  int64_t v_stride_token, v_stride_head;
+  int dtype;
+} omni_read_cache_args;
+int omni_read_cache(const omni_read_cache_args* args, omni_stream_t stream);
 
 /*
  * omni_prompt_attention: attention of packed sequences. Sequence s has the queries starts[s] ..

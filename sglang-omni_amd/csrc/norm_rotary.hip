@@ -321,7 +321,7 @@ struct ReadParams {
   void* dst[2];
   int64_t dst_token[2], dst_head[2];
   int64_t items;  // tokens * kv_heads * chunks
-  int kv_heads, chunks, dim;
+  int kv_heads, chunks;
 };
 
 // A lane takes 16 values of a key row and of its value row: 16 or 32 bytes of each.
@@ -467,38 +467,36 @@ extern "C" int omni_norm_rotary(const omni_norm_rotary_args* a, omni_stream_t st
   }
 }
 
-extern "C" int omni_read_cache(const omni_kv_cache* cache, const void* slots, int slots_dtype,
-                               int64_t slots_stride, int64_t tokens, void* k, int64_t k_stride_token,
-                               int64_t k_stride_head, void* v, int64_t v_stride_token,
-                               int64_t v_stride_head, int dtype, omni_stream_t stream) {
+extern "C" int omni_read_cache(const omni_read_cache_args* a, omni_stream_t stream) {
   ReadParams p{};
-  if (!cache || tokens < 0 || !index_type(slots_dtype) || cache->kv_heads < 1 || cache->dim < 16 ||
-      cache->dim % 16 || cache->kv_heads > 65536 || cache->dim > 65536 || !cache_view(*cache, 16, &p.cache))
+  if (!a || !a->cache || a->tokens < 0 || !index_type(a->slots_dtype)) return OMNI_ERR_INVALID_ARG;
+  const omni_kv_cache& cache = *a->cache;
+  if (cache.kv_heads < 1 || cache.dim < 16 || cache.dim % 16 || cache.kv_heads > 65536 ||
+      cache.dim > 65536 || !cache_view(cache, 16, &p.cache))
     return OMNI_ERR_INVALID_ARG;
-  if (dtype != OMNI_DTYPE_F32 && dtype != OMNI_DTYPE_BF16 && dtype != OMNI_DTYPE_F16)
+  if (a->dtype != OMNI_DTYPE_F32 && a->dtype != OMNI_DTYPE_BF16 && a->dtype != OMNI_DTYPE_F16)
     return OMNI_ERR_INVALID_ARG;
-  if (tokens == 0) return OMNI_OK;
-  const int size = dtype == OMNI_DTYPE_F32 ? 4 : 2;
-  if (!slots || !aligned_to(slots, slots_dtype == OMNI_DTYPE_I64 ? 8 : 4) || !k || !v ||
-      !aligned_to(k, size) || !aligned_to(v, size))
+  if (a->tokens == 0) return OMNI_OK;
+  const int size = a->dtype == OMNI_DTYPE_F32 ? 4 : 2;
+  if (!a->slots || !aligned_to(a->slots, a->slots_dtype == OMNI_DTYPE_I64 ? 8 : 4) || !a->k || !a->v ||
+      !aligned_to(a->k, size) || !aligned_to(a->v, size))
     return OMNI_ERR_INVALID_ARG;
-  p.slots = slots;
-  p.slots64 = slots_dtype == OMNI_DTYPE_I64;
-  p.slots_stride = slots_stride;
-  p.dst[0] = k;
-  p.dst[1] = v;
-  p.dst_token[0] = k_stride_token;
-  p.dst_token[1] = v_stride_token;
-  p.dst_head[0] = k_stride_head;
-  p.dst_head[1] = v_stride_head;
-  p.kv_heads = (int)cache->kv_heads;
-  p.chunks = (int)(cache->dim / 16);
-  p.dim = (int)cache->dim;
-  p.items = tokens * p.kv_heads * p.chunks;
+  p.slots = a->slots;
+  p.slots64 = a->slots_dtype == OMNI_DTYPE_I64;
+  p.slots_stride = a->slots_stride;
+  p.dst[0] = a->k;
+  p.dst[1] = a->v;
+  p.dst_token[0] = a->k_stride_token;
+  p.dst_token[1] = a->v_stride_token;
+  p.dst_head[0] = a->k_stride_head;
+  p.dst_head[1] = a->v_stride_head;
+  p.kv_heads = (int)cache.kv_heads;
+  p.chunks = (int)(cache.dim / 16);
+  p.items = a->tokens * p.kv_heads * p.chunks;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  switch (cache->dtype) {
-    case OMNI_DTYPE_FP8_E4M3: return launch_read_as<uint8_t>(p, dtype, s);
-    case OMNI_DTYPE_BF16: return launch_read_as<__bf16>(p, dtype, s);
-    default: return launch_read_as<_Float16>(p, dtype, s);
+  switch (cache.dtype) {
+    case OMNI_DTYPE_FP8_E4M3: return launch_read_as<uint8_t>(p, a->dtype, s);
+    case OMNI_DTYPE_BF16: return launch_read_as<__bf16>(p, a->dtype, s);
+    default: return launch_read_as<_Float16>(p, a->dtype, s);
   }
 }

@@ -423,7 +423,7 @@ int launch_dim(const PagedParams& p, hipStream_t stream) {
 extern "C" int omni_paged_attention(const omni_paged_args* a, omni_stream_t stream) {
   if (!a || !a->cache || a->batch < 0 || a->heads < 1 || a->cache->kv_heads < 1 ||
       a->heads % a->cache->kv_heads || a->heads > 65535 || a->cache->dim < 16 || a->cache->dim % 16 ||
-      a->table_columns < 0 || a->max_length < 0 || !(a->scale > 0.f) || !(a->scale <= 3.0e38f) ||
+      a->table_columns < 0 || a->max_length < 0 || !(a->scale > 0.f) || !(a->scale <= 1e30f) ||
       (a->dtype != OMNI_DTYPE_BF16 && a->dtype != OMNI_DTYPE_F16) ||
       (a->cache->dtype != OMNI_DTYPE_FP8_E4M3 && a->cache->dtype != a->dtype) ||
       (a->lengths_dtype != OMNI_DTYPE_I32 && a->lengths_dtype != OMNI_DTYPE_I64))

@@ -604,7 +604,7 @@ extern "C" int64_t omni_prompt_plan(int64_t tokens, int64_t key_tokens, int64_t 
 extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t stream) {
   if (!a || a->tokens < 0 || a->key_tokens < 0 || a->sequences < 0 || a->heads < 1 || a->kv_heads < 1 ||
       a->heads % a->kv_heads || a->heads > 65536 || a->dim < 8 || a->dim % 8 || !(a->scale > 0.f) ||
-      !(a->scale <= 3.0e38f) || a->sequences > 0x7ffffff0LL ||
+      !(a->scale <= 1e30f) || a->sequences > 0x7ffffff0LL ||
       (a->dtype != OMNI_DTYPE_BF16 && a->dtype != OMNI_DTYPE_F16) ||
       (a->starts_dtype != OMNI_DTYPE_I32 && a->starts_dtype != OMNI_DTYPE_I64))
     return OMNI_ERR_INVALID_ARG;

@@ -390,6 +390,25 @@ class NormRotaryArgs(ctypes.Structure):
     ]
 
 
+class ReadCacheArgs(ctypes.Structure):
+    """Mirror of ``omni_read_cache_args`` in include/omni_codec.h."""
+
+    _fields_ = [
+        ("cache", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("slots_dtype", ctypes.c_int),
+        ("slots_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v", ctypes.c_void_p),
+        ("v_stride_token", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+    ]
+
+
 class PromptArgs(ctypes.Structure):
     """Mirror of ``omni_prompt_args`` in include/omni_codec.h."""
 
@@ -466,6 +485,7 @@ pack_rotary = _packer(RotaryArgs)
 pack_logits = _packer(LogitsArgs)
 pack_kv_cache = _packer(KvCacheStruct)
 pack_norm_rotary = _packer(NormRotaryArgs)
+pack_read_cache = _packer(ReadCacheArgs)
 pack_prompt = _packer(PromptArgs)
 pack_paged = _packer(PagedArgs)
 BLOCK_FP8_FEW_ROWS = 16
@@ -546,7 +566,7 @@ SIGNATURES: dict[str, list] = {
     "omni_rotary": [ctypes.c_char_p, _PTR],
     "omni_adjust_logits": [ctypes.c_char_p, _PTR],
     "omni_norm_rotary": [ctypes.c_char_p, _PTR],
-    "omni_read_cache": [_PTR, _PTR, _INT, _I64, _I64, _PTR, _I64, _I64, _PTR, _I64, _I64, _INT, _PTR],
+    "omni_read_cache": [ctypes.c_char_p, _PTR],
     "omni_prompt_plan": [_I64, _I64, _I64, _I64, _I64, _I64, _INT, ctypes.POINTER(_INT)],
     "omni_prompt_attention": [ctypes.c_char_p, _PTR],
     "omni_paged_attention": [ctypes.c_char_p, _PTR],

@@ -49,15 +49,17 @@ class PagedKvCache:
         if strides[3] != 1 or strides[0] % each or strides[1] % each or strides[2] % each \
                 or keys.data_ptr() % 16 or values.data_ptr() % 16:
             raise ValueError("a cache's rows must be contiguous and 16-byte aligned")
-        scales = (0, 0, 0, 0, 0)
         if dtype is _E4M3:
-            for t in (key_scale, value_scale):
-                if t is None or t.dtype is not torch.float32 or t.shape != shape[:3] \
-                        or t.get_device() != index or t.stride() != key_scale.stride():
-                    raise ValueError(f"an E4M3 cache has float32 scales {list(shape[:3])} of the same "
-                                     "strides for keys and values")
+            if key_scale is None or value_scale is None or key_scale.dtype is not torch.float32 \
+                    or value_scale.dtype is not torch.float32 or key_scale.get_device() != index \
+                    or value_scale.get_device() != index or key_scale.shape != shape[:3] \
+                    or value_scale.shape != shape[:3] or key_scale.stride() != value_scale.stride():
+                raise ValueError(f"an E4M3 cache has float32 scales {list(shape[:3])} of the same "
+                                 "strides for keys and values")
             scales = (key_scale.data_ptr(), value_scale.data_ptr(), *key_scale.stride())
-        elif key_scale is not None or value_scale is not None:
+        elif key_scale is None and value_scale is None:
+            scales = (0, 0, 0, 0, 0)
+        else:
             raise ValueError("scales go with E4M3 rows")
         self._keys, self._values = keys, values
         self._key_scale, self._value_scale = key_scale, value_scale
@@ -134,6 +136,15 @@ def write_kv_cache(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor,
         N.check(status, "omni_norm_rotary")
 
 
+def _read_into(t: torch.Tensor, name: str, tokens: int, dtype: torch.dtype,
+               cache: PagedKvCache) -> tuple[int, int]:
+    strides = _rows(t, name, cache)
+    if t.shape[0] != tokens or t.dtype is not dtype or t.get_device() != cache.index:
+        raise ValueError(f"{name} must be [{tokens}, {cache.kv_heads}, {cache.dim}] of {dtype} on the "
+                         "cache's GPU")
+    return strides
+
+
 def read_kv_cache(cache: PagedKvCache, slots: torch.Tensor, *, dtype: torch.dtype | None = None,
                   k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None
                   ) -> tuple[torch.Tensor, torch.Tensor]:
@@ -151,21 +162,25 @@ def read_kv_cache(cache: PagedKvCache, slots: torch.Tensor, *, dtype: torch.dtyp
     if dtype not in _FLOATS:
         raise ValueError("rows are read as bf16, f16 or f32")
     tokens = slots.shape[0] if slots.dim() == 1 else -1
-    at = _slots(slots, tokens, index)
-    shape = (tokens, cache.kv_heads, cache.dim)
+    slots_ptr, slots_dtype, slots_stride = _slots(slots, tokens, index)
+    kv_heads, dim = cache.kv_heads, cache.dim
+    k_token = v_token = kv_heads * dim
+    k_head = v_head = dim
     if k_out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=slots.device)
+        k_out = torch.empty(tokens, kv_heads, dim, dtype=dtype, device=slots.device)
+    else:
+        k_token, k_head = _read_into(k_out, "k_out", tokens, dtype, cache)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=slots.device)
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
-            raise ValueError(f"{name} must be {list(shape)} of {dtype} on the cache's GPU")
-    k_strides, v_strides = _rows(k_out, "k_out", cache), _rows(v_out, "v_out", cache)
+        v_out = torch.empty(tokens, kv_heads, dim, dtype=dtype, device=slots.device)
+    else:
+        v_token, v_head = _read_into(v_out, "v_out", tokens, dtype, cache)
+    args = N.pack_read_cache(cache.address, slots_ptr, slots_dtype, slots_stride, tokens,
+                             k_out.data_ptr(), k_token, k_head, v_out.data_ptr(), v_token, v_head,
+                             _CODES[dtype])
     global _read
     if _read is None:
         _read = N.load_library().omni_read_cache
-    status = N.launch_on(index, _read, cache.address, *at[:2], at[2], tokens, k_out.data_ptr(),
-                         *k_strides, v_out.data_ptr(), *v_strides, _CODES[dtype])
+    status = N.launch_on(index, _read, args)
     if status:
         N.check(status, "omni_read_cache")
     return k_out, v_out

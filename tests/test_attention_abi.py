@@ -14,6 +14,7 @@ from tests.test_operator_abi import HEADER, _header_fields
 
 STRUCTS = [("omni_kv_cache", N.KvCacheStruct, N.pack_kv_cache),
            ("omni_norm_rotary_args", N.NormRotaryArgs, N.pack_norm_rotary),
+           ("omni_read_cache_args", N.ReadCacheArgs, N.pack_read_cache),
            ("omni_prompt_args", N.PromptArgs, N.pack_prompt),
            ("omni_paged_args", N.PagedArgs, N.pack_paged)]
 
@@ -59,7 +60,8 @@ def test_refused_before_any_launch():
     """The C entry points check their arguments before the GPU is asked for anything: every call here
     has one thing wrong, and pointers that no launch could have read."""
     lib = N.load_library()
-    entries = {"omni_norm_rotary_args": lib.omni_norm_rotary, "omni_prompt_args": lib.omni_prompt_attention,
+    entries = {"omni_norm_rotary_args": lib.omni_norm_rotary,
+               "omni_read_cache_args": lib.omni_read_cache, "omni_prompt_args": lib.omni_prompt_attention,
                "omni_paged_args": lib.omni_paged_attention}
     for name, args, pack in STRUCTS[1:]:
         assert entries[name](None, None) == N.INVALID_ARG
@@ -131,15 +133,16 @@ def test_refused_before_any_launch():
         assert heads_status(held) == N.INVALID_ARG, held
     assert heads_status(dim=514) == N.UNSUPPORTED
 
-    def read_status(held=None, slots=4096, kind=N.DTYPE_I64, tokens=8, k=4096, dtype=N.DTYPE_BF16):
-        return lib.omni_read_cache(cache(**(held or {})), slots, kind, 1, tokens, k, 32, 16, 4096, 32, 16,
-                                   dtype, None)
+    read = dict(slots=4096, slots_dtype=N.DTYPE_I64, slots_stride=1, tokens=8, k=4096, k_stride_token=32,
+                k_stride_head=16, v=4096, v_stride_token=32, v_stride_head=16, dtype=N.DTYPE_BF16)
+
+    def read_status(held=None, **kw):
+        fields = {**read, "cache": cache(**(held or {})), **kw}
+        return lib.omni_read_cache(N.pack_read_cache(*_fields(N.ReadCacheArgs, **fields)), None)
 
     assert read_status(tokens=0) == N.OK
-    assert lib.omni_read_cache(None, 4096, N.DTYPE_I64, 1, 0, 4096, 32, 16, 4096, 32, 16, 0, None) \
-        == N.INVALID_ARG
-    for kw in ({"held": {"dim": 24}}, {"held": {"keys": 4104}}, {"slots": 4}, {"kind": N.DTYPE_F32},
-               {"tokens": -1}, {"k": 0}, {"k": 4097}, {"dtype": N.DTYPE_FP8_E4M3}):
+    for kw in ({"held": {"dim": 24}}, {"held": {"keys": 4104}}, {"slots": 4}, {"slots_dtype": N.DTYPE_F32},
+               {"tokens": -1}, {"cache": 0}, {"k": 0}, {"k": 4097}, {"dtype": N.DTYPE_FP8_E4M3}):
         assert read_status(**kw) == N.INVALID_ARG, kw
 
 
