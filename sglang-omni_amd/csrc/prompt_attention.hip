@@ -293,28 +293,58 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
       }
   };
   // and its values: one that some of these rows do not see may be an infinity or a NaN, and zero times
-  // it is one too. Such a tile's sum over zeros is not zero.
+  // it is one too, so that its keys' sum over zeros is not zero. LONG, whose registers are all in use, looks
+  // the tile over at once; else 16 keys at a time, those that only some of the rows see, and those that
+  // none sees are passed over (taken so, LONG spills: 24 x 350 tokens of 16 heads 45 -> 52 us).
   auto accumulate_seen = [&](int first_key, int stage, const typename O::x8 (&w)[kSteps])
                              __attribute__((always_inline)) {
+    uint32_t bad = 0;
+    auto any = [&](const f32x16& zeros) __attribute__((always_inline)) {
+      bool some = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) some |= zeros[i] != 0.f;
+      return __ballot(some) != 0;
+    };
     f32x16 zeros;
+    if constexpr (LONG) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) zeros[i] = 0.f;
-    const typename O::x8 none{};
+      for (int i = 0; i < 16; ++i) zeros[i] = 0.f;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+      for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int c = 0; c < kSteps; ++c) zeros = O::mfma32(v_operand(stage, c, d), none, zeros);
-    bool bad = false;
+        for (int c = 0; c < kSteps; ++c) zeros = O::mfma32(v_operand(stage, c, d), typename O::x8{}, zeros);
+      if (any(zeros))
+        bad = (1u << kSteps) - 1;
+      else
+        accumulate(stage, w);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) bad |= zeros[i] != 0.f;
-    if (__ballot(bad) == 0) {
-      accumulate(stage, w);
-      return;
+      for (int c = 0; c < kSteps; ++c) {
+        const int key = first_key + c * 16;
+        if (key >= seen_most) continue;
+        typename O::x8 v[D / 32];
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) v[d] = v_operand(stage, c, d);
+        if (key + 16 > seen_least) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) zeros[i] = 0.f;
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) zeros = O::mfma32(v[d], typename O::x8{}, zeros);
+          if (any(zeros)) {
+            bad |= 1u << c;
+            continue;
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) o[d] = O::mfma32(v[d], w[c], o[d]);
+      }
     }
+    if (bad == 0) return;
     // each key's contribution on its own, added where it is seen; rare, so a loop of little code
 #pragma unroll 1
     for (int e = 0; e < kKeys; ++e) {
       const int c = e / 16, key = first_key + c * 16 + (e % 8 / 4) * 8 + (e % 16 / 8) * 4 + e % 4;
+      if ((bad >> c & 1) == 0) continue;
       const bool mine = half == e % 16 / 8;
       typename O::x8 wc = w[0];
 #pragma unroll
