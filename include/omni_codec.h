@@ -1068,12 +1068,11 @@ int omni_prompt_attention(const omni_prompt_args* args, omni_stream_t stream);
  * operands; outputs rounded once. A row's bits depend on its own sequence alone.
  *
  * Strides of q and out in elements, multiples of 8, pointers and the cache's rows 16-byte aligned; dim a
- * multiple of 16 up to 256; batch up to 65535; scale positive. workspace: with L = OMNI_PAGED_LEAST_CHUNK
- * and c = ceil(max_length / L) up to 8, else max(8, ceil(max_length / 2 L)) up to 32, else max(32,
- * ceil(max_length / OMNI_PAGED_MOST_CHUNK)), at least batch * heads * c * (dim + 2) * 4 bytes, 16-byte
- * aligned; none for a max_length up to 2 L. batch = 0 does nothing.
+ * multiple of 16 up to 256; batch up to 65535; scale positive. workspace: omni_paged_workspace(batch,
+ * heads, kv_heads, dim, max_length) bytes, 16-byte aligned. batch = 0 does nothing.
  */
-enum { OMNI_PAGED_LEAST_CHUNK = 256, OMNI_PAGED_MOST_CHUNK = 1024 };
+int64_t omni_paged_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                             int64_t max_length);
 typedef struct omni_paged_args {
   const void* q;
   int64_t q_stride_row, q_stride_head;

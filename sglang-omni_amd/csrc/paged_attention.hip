@@ -16,6 +16,7 @@
 // kernel, V read transposed from shared memory. bf16 weights are held as a sum of two bf16 numbers, 16
 // bits of each weight: the matrix cores have nothing else to do here. 8-bit rows widen exactly; the keys'
 // scales multiply the scores and the values' the weights.
+#include <initializer_list>
 #include <type_traits>
 
 #include "attention.h"
@@ -42,17 +43,21 @@ struct PagedParams {
 constexpr int kKeys = 32;  // of a tile
 constexpr int kWaves = 4;
 constexpr float kLazy = 6.f;
-constexpr int kLeastChunk = OMNI_PAGED_LEAST_CHUNK, kMostChunk = OMNI_PAGED_MOST_CHUNK;
+constexpr int kLeastChunk = 256, kMostChunk = 1024;
 
-// The keys of a chunk. Short chunks spread one stream over the chip, long ones have fewer starts and parts:
-// with 256, 512 and 1024 for all lengths 1 x 2000 took 13.4, 16.8 and 25.2 us, 1 x 9000 23.4, 23.7 and 30.9,
-// 64 up to 5000 174, 160 and 158, 2 x 131072 176, 175 and 170 (E4M3). Up to 512 keys are one chunk, which
-// needs no second launch.
-OMNI_DEVICE int chunk_of(int length) {
-  return length <= 2 * kLeastChunk    ? 2 * kLeastChunk
-         : length <= 8 * kLeastChunk  ? kLeastChunk
-         : length <= 64 * kLeastChunk ? 2 * kLeastChunk
-                                      : kMostChunk;
+// The keys of a chunk, by a sequence's length and the workgroups that share its chunks (a key head's 16
+// query heads each). Short chunks spread one stream over the chip, long ones have fewer starts and parts:
+// with 256, 512 and 1024 for all lengths and 8 key heads 1 x 2000 took 13.4, 16.8 and 25.2 us, 1 x 9000 23.4,
+// 23.7 and 30.9, 64 up to 5000 174, 160 and 158, 2 x 131072 176, 175 and 170 (E4M3). Fewer heads leave more
+// of the chip to the chunks. Up to 512 keys are one chunk, which needs no second launch.
+__host__ __device__ inline int units_of(int kv_heads, int head_tiles) {
+  return kv_heads * head_tiles < 8 ? kv_heads * head_tiles : 8;
+}
+__host__ __device__ inline int chunk_of(int64_t length, int units) {
+  return length <= 2 * kLeastChunk            ? 2 * kLeastChunk
+         : length * units <= 64 * kLeastChunk ? kLeastChunk
+         : length * units <= 512 * kLeastChunk ? 2 * kLeastChunk
+                                              : kMostChunk;
 }
 
 // The keys that sequence b's query sees: within the table's room and max_length.
@@ -122,7 +127,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
   const int kv_head = blockIdx.y / p.head_tiles, head_tile = blockIdx.y % p.head_tiles;
   const int b = blockIdx.z;
   const int length = length_of(p, b);
-  const int size = chunk_of(length);
+  const int size = chunk_of(length, units_of(p.kv_heads, p.head_tiles));
   const int chunks = (length + size - 1) / size;
   if (chunk > 0 && chunk >= chunks) return;
   const int first = chunk * size, count = length - first < size ? length - first : size;
@@ -358,7 +363,8 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
   const int heads = p.kv_heads * p.group;
   const int b = blockIdx.x / heads, head = blockIdx.x % heads;
   const int length = length_of(p, b);
-  const int size = chunk_of(length), chunks = (length + size - 1) / size;
+  const int size = chunk_of(length, units_of(p.kv_heads, p.head_tiles));
+  const int chunks = (length + size - 1) / size;
   if (chunks <= 1) return;
   const int64_t at = ((int64_t)b * heads + head) * p.chunks;
   const float* stats = p.parts + (int64_t)p.batch * heads * p.chunks * p.dim + at * 2;
@@ -373,13 +379,30 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
   f32x4 o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int c = part; c < chunks; c += 16) {
-    const float keep = __builtin_amdgcn_exp2f(stats[2 * c] - m_use);
-    l = __builtin_fmaf(stats[2 * c + 1], keep, l);
+  // a quarter-wave's chunks four at a time, so that their loads are on their way together; one past the
+  // last is the last one again, and counts nothing
+  for (int first = part; first < chunks; first += 64) {
+    float keep[4], sum[4];
+    f32x4 x[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i * 64 + quad * 4 < p.dim)
-        o[i] += *reinterpret_cast<const f32x4*>(p.parts + (at + c) * p.dim + i * 64 + quad * 4) * keep;
+    for (int j = 0; j < 4; ++j) {
+      const int c = first + j * 16 < chunks ? first + j * 16 : chunks - 1;
+      keep[j] = first + j * 16 < chunks ? stats[2 * c] : -__builtin_inff();
+      sum[j] = stats[2 * c + 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i * 64 + quad * 4 < p.dim)
+          x[j][i] = *reinterpret_cast<const f32x4*>(p.parts + (at + c) * p.dim + i * 64 + quad * 4);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (first + j * 16 >= chunks) break;
+      const float weight = __builtin_amdgcn_exp2f(keep[j] - m_use);
+      l = __builtin_fmaf(sum[j], weight, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i * 64 + quad * 4 < p.dim) o[i] += x[j][i] * weight;
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(sums[part][i * 16 + quad]) = o[i];
@@ -418,7 +441,26 @@ int launch_dim(const PagedParams& p, hipStream_t stream) {
   return launch_paged<T, H, 256>(p, stream);
 }
 
+// The most chunks of a length up to `bound`: those of the last length of each chunk size.
+int64_t most_chunks(int64_t bound, int kv_heads, int head_tiles) {
+  const int units = units_of(kv_heads, head_tiles);
+  int64_t most = 1;
+  for (int64_t last : {(int64_t)64 * kLeastChunk / units, (int64_t)512 * kLeastChunk / units, bound}) {
+    const int64_t length = last < bound ? last : bound, size = chunk_of(length, units);
+    const int64_t chunks = (length + size - 1) / size;
+    most = chunks > most ? chunks : most;
+  }
+  return most;
+}
+
 }  // namespace
+
+extern "C" int64_t omni_paged_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                                        int64_t max_length) {
+  if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65535 || dim < 1) return 0;
+  const int64_t chunks = most_chunks(max_length, (int)kv_heads, (int)((heads / kv_heads + 15) / 16));
+  return chunks > 1 ? batch * heads * chunks * (dim + 2) * 4 : 0;
+}
 
 extern "C" int omni_paged_attention(const omni_paged_args* a, omni_stream_t stream) {
   if (!a || !a->cache || a->batch < 0 || a->heads < 1 || a->cache->kv_heads < 1 ||
@@ -442,12 +484,7 @@ extern "C" int omni_paged_attention(const omni_paged_args* a, omni_stream_t stre
   const int64_t kv_heads = a->cache->kv_heads, group = a->heads / kv_heads;
   const int64_t tiles = (group + 15) / 16;
   if (kv_heads * tiles > 65535 || a->batch * a->heads > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
-  // the most chunks of a length up to max_length: one up to 512, at most 8 up to 2048, then 32 up to 16384
-  auto pieces = [&](int64_t size) { return (a->max_length + size - 1) / size; };
-  int64_t chunks = pieces(kLeastChunk);
-  if (chunks > 8) chunks = pieces(2 * kLeastChunk) > 8 ? pieces(2 * kLeastChunk) : 8;
-  if (chunks > 32) chunks = pieces(kMostChunk) > 32 ? pieces(kMostChunk) : 32;
-  if (a->max_length <= 2 * kLeastChunk) chunks = 1;
+  const int64_t chunks = most_chunks(a->max_length, (int)kv_heads, (int)tiles);
   if (chunks > 1 && (!a->workspace || !aligned_to(a->workspace, 16) ||
                      a->workspace_bytes < a->batch * a->heads * chunks * (a->cache->dim + 2) * 4))
     return OMNI_ERR_INVALID_ARG;

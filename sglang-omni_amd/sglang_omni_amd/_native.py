@@ -489,7 +489,6 @@ pack_read_cache = _packer(ReadCacheArgs)
 pack_prompt = _packer(PromptArgs)
 pack_paged = _packer(PagedArgs)
 BLOCK_FP8_FEW_ROWS = 16
-PAGED_LEAST_CHUNK, PAGED_MOST_CHUNK = 256, 1024
 
 GEMM_STORE, GEMM_SILU_MUL, GEMM_GELU, GEMM_SCALED_RESIDUAL = 0, 1, 2, 3
 NORM_RMS, NORM_LAYER = 0, 1
@@ -569,9 +568,11 @@ SIGNATURES: dict[str, list] = {
     "omni_read_cache": [ctypes.c_char_p, _PTR],
     "omni_prompt_plan": [_I64, _I64, _I64, _I64, _I64, _I64, _INT, ctypes.POINTER(_INT)],
     "omni_prompt_attention": [ctypes.c_char_p, _PTR],
+    "omni_paged_workspace": [_I64, _I64, _I64, _I64, _I64],
     "omni_paged_attention": [ctypes.c_char_p, _PTR],
 }
-_RESTYPES = {"omni_codec_error_string": ctypes.c_char_p, "omni_prompt_plan": _I64}
+_RESTYPES = {"omni_codec_error_string": ctypes.c_char_p, "omni_prompt_plan": _I64,
+             "omni_paged_workspace": _I64}
 
 _lib: ctypes.CDLL | None = None
 

@@ -14,7 +14,7 @@ _INDEXES = (torch.int64, torch.int32)
 _E4M3 = torch.float8_e4m3fn
 _CODES = N.TORCH_TO_OMNI
 _prompt = _plan = None  # the entry points, bound at the first call
-_paged = None
+_paged = _workspace = None
 
 
 def _heads(t: torch.Tensor, name: str) -> tuple[int, int]:
@@ -106,18 +106,6 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     return out
 
 
-def _workspace_bytes(rows: int, dim: int, max_length: int) -> int:
-    """What omni_paged_attention needs for the parts of `rows` heads of all sequences."""
-    if max_length <= 2 * N.PAGED_LEAST_CHUNK:
-        return 0
-    chunks = -(-max_length // N.PAGED_LEAST_CHUNK)
-    if chunks > 8:
-        chunks = max(8, -(-max_length // (2 * N.PAGED_LEAST_CHUNK)))
-        if chunks > 32:
-            chunks = max(32, -(-max_length // N.PAGED_MOST_CHUNK))
-    return rows * chunks * (dim + 2) * 4
-
-
 def paged_attention(q: torch.Tensor, cache: PagedKvCache, table: torch.Tensor, lengths: torch.Tensor,
                     *, scale: float | None = None, max_length: int | None = None,
                     out: torch.Tensor | None = None) -> torch.Tensor:
@@ -162,16 +150,17 @@ def paged_attention(q: torch.Tensor, cache: PagedKvCache, table: torch.Tensor, l
         out_row, out_head = _heads(out, "out")
         if out.shape != q.shape or out.dtype is not dtype or out.get_device() != index:
             raise ValueError("out must be like q")
-    needed = _workspace_bytes(batch * heads, dim, max_length)
+    global _paged, _workspace
+    if _paged is None:
+        lib = N.load_library()
+        _paged, _workspace = lib.omni_paged_attention, lib.omni_paged_workspace
+    needed = _workspace(batch, heads, cache.kv_heads, dim, max_length)
     workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
     args = N.pack_paged(
         q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head, _CODES[dtype], batch, heads,
         cache.address, table.data_ptr(), table.stride(0), columns, lengths.data_ptr(),
         _CODES[lengths.dtype], max_length, _scale(scale, dim),
         0 if workspace is None else workspace.data_ptr(), needed)
-    global _paged
-    if _paged is None:
-        _paged = N.load_library().omni_paged_attention
     status = N.launch_on(index, _paged, args)
     if status:
         N.check(status, "omni_paged_attention")

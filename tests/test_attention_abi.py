@@ -3,14 +3,11 @@ header's, and refusals before any launch."""
 
 from __future__ import annotations
 
-import re
-
 import pytest
 import torch
 
 from sglang_omni_amd import _native as N
-from sglang_omni_amd.kernels import attention
-from tests.test_operator_abi import HEADER, _header_fields
+from tests.test_operator_abi import _header_fields
 
 STRUCTS = [("omni_kv_cache", N.KvCacheStruct, N.pack_kv_cache),
            ("omni_norm_rotary_args", N.NormRotaryArgs, N.pack_norm_rotary),
@@ -28,28 +25,26 @@ def test_fields_mirror_the_header(name, args, pack):
     assert struct[:len(packed)] == packed and len(struct) - len(packed) < 8
 
 
-def test_constants_match_the_header():
-    text = HEADER.read_text()
-    for name, value in {"OMNI_PAGED_LEAST_CHUNK": N.PAGED_LEAST_CHUNK,
-                        "OMNI_PAGED_MOST_CHUNK": N.PAGED_MOST_CHUNK}.items():
-        assert int(re.search(rf"\b{name}\s*=\s*(\d+)", text).group(1)) == value, name
-
-
-def _chunks(length):
+def _chunks(length, units):
     """The chunks of a sequence, by the kernel's rule."""
-    least, most = N.PAGED_LEAST_CHUNK, N.PAGED_MOST_CHUNK
-    if length <= 2 * least:
+    if length <= 512:
         return 1
-    size = least if length <= 8 * least else 2 * least if length <= 64 * least else most
+    size = 256 if length * units <= 64 * 256 else 512 if length * units <= 512 * 256 else 1024
     return -(-length // size)
 
 
-def test_workspace_holds_the_parts_of_every_length():
-    for bound in [0, 1, 255, 256, 257, 512, 513, 2048, 2049, 4096, 8191, 8192, 8193, 16384, 16385, 32768, 32769, 40000, 131072]:
-        held = attention._workspace_bytes(3, 16, bound) // (3 * 18 * 4)
-        for length in {0, 1, 256, 257, 512, 513, 2048, 2049, 8192, 8193, 16384, 16385, bound}:
+@pytest.mark.parametrize("heads,kv", [(8, 8), (32, 8), (64, 32), (14, 2), (20, 1), (6, 3), (40, 1), (5, 5)])
+def test_workspace_holds_the_parts_of_every_length(heads, kv):
+    lib = N.load_library()
+    units = min(kv * -(-heads // kv // 16), 8)
+    edges = [0, 1, 256, 257, 512, 513, 64 * 256 // units, 64 * 256 // units + 1, 512 * 256 // units,
+             512 * 256 // units + 1, 40000, 131072, 10 ** 6]
+    for bound in edges:
+        held = lib.omni_paged_workspace(3, heads, kv, 16, bound) // (3 * heads * 18 * 4)
+        for length in edges:
             if length <= bound:
-                assert _chunks(length) <= max(held, 1), (bound, length)
+                assert _chunks(length, units) <= max(held, 1), (bound, length)
+        assert (held == 0) == (bound <= 512)
 
 
 def _fields(args, **values):
