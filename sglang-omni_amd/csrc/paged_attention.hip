@@ -5,7 +5,9 @@
 // for every head, the heads of a group over one key head. Rows of E4M3 count scale_j times their bytes.
 // A sequence without keys is zero. Keys on a page outside the cache are left out.
 //
-// The cache is read once, and that bounds it. A sequence's keys are cut into chunks whose size follows
+// The cache is read once, and that bounds it: 2 x 131072 keys of 8 heads of 128 in 100 us in 8 bits (5.5
+// TB/s; a plain read of 1 GiB 6.3, a copy 5.06) and 183 in bf16 (5.9), 64 streams up to 5000 in 148 (4.95);
+// one stream of 300 in 7.7, a chain of loads: length, table, rows. A sequence's keys are cut into chunks whose size follows
 // from its length alone, so that a row's bits do not depend on the batch; a workgroup takes a chunk of a
 // key head for up to 16 query heads, its four waves every fourth tile of 32 keys each, with their own
 // running maximum and sum, joined through shared memory. One chunk is the result; several are joined by
@@ -47,9 +49,10 @@ constexpr int kLeastChunk = 256, kMostChunk = 1024;
 
 // The keys of a chunk, by a sequence's length and the workgroups that share its chunks (a key head's 16
 // query heads each). Short chunks spread one stream over the chip, long ones have fewer starts and parts:
-// with 256, 512 and 1024 for all lengths and 8 key heads 1 x 2000 took 13.4, 16.8 and 25.2 us, 1 x 9000 23.4,
-// 23.7 and 30.9, 64 up to 5000 174, 160 and 158, 2 x 131072 176, 175 and 170 (E4M3). Fewer heads leave more
-// of the chip to the chunks. Up to 512 keys are one chunk, which needs no second launch.
+// with 256, 512 and 1024 for all lengths and 8 key heads 1 x 2000 takes 10.4, 12.3 and 17.1 us, 1 x 9000 14.1,
+// 14.3 and 19.7, 64 up to 5000 157, 147 and 140, 2 x 131072 127, 116 and 103 (E4M3); over 2 key heads 9 up to
+// 20000 15.5, 16.3 and 18.4: fewer heads leave more of the chip to the chunks. Up to 512 keys are one chunk,
+// which needs no second launch.
 __host__ __device__ inline int units_of(int kv_heads, int head_tiles) {
   return kv_heads * head_tiles < 8 ? kv_heads * head_tiles : 8;
 }
@@ -189,8 +192,8 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
       }
     }
   };
-  // The values past the caches: nothing reads them again. (A line of keys is read in two halves.) 2 x 131072
-  // in 8 bits 127 -> 108 us, 128 x 1000 115 -> 93; the keys so too 122 and 110.
+  // The values past the caches: nothing reads them again. (A line of keys is read in two halves.) When it was
+  // done 2 x 131072 in 8 bits went from 127 to 108 us, 128 x 1000 from 115 to 93; with the keys so too 122 and 110.
   auto load_values_of = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < kVLoads; ++s) {
@@ -358,8 +361,9 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
 
 // The chunks of a (sequence, head) joined: a workgroup of 4 waves, a quarter-wave to a row of up to 64
 // dimensions (4 a lane), so 16 chunks at a time, their sums joined in a fixed order.
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
+  constexpr int kQuads = D / 64;  // a lane's, 64 dimensions apart
   const int heads = p.kv_heads * p.group;
   const int b = blockIdx.x / heads, head = blockIdx.x % heads;
   const int length = length_of(p, b);
@@ -368,7 +372,7 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
   if (chunks <= 1) return;
   const int64_t at = ((int64_t)b * heads + head) * p.chunks;
   const float* stats = p.parts + (int64_t)p.batch * heads * p.chunks * p.dim + at * 2;
-  __shared__ float sums[16][64 + 1][4];
+  __shared__ float sums[16][D / 4 + 1][4];
   const int lane = threadIdx.x & 63, part = threadIdx.x >> 4, quad = threadIdx.x & 15;
   float m = -__builtin_inff();
   for (int c = lane; c < chunks; c += 64) m = fmaxf(m, stats[2 * c]);
@@ -376,37 +380,44 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
   for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
   const float m_use = m == -__builtin_inff() ? 0.f : m;
   float l = 0.f;
-  f32x4 o[4];
+  f32x4 o[kQuads];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // a quarter-wave's chunks four at a time, so that their loads are on their way together; one past the
-  // last is the last one again, and counts nothing
-  for (int first = part; first < chunks; first += 64) {
-    float keep[4], sum[4];
-    f32x4 x[4][4];
+  for (int i = 0; i < kQuads; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // A quarter-wave's chunks, where there are several up to four at a time, so that their loads are on their way
+  // together; one past the last is the last one again, and counts nothing.
+  auto add = [&](auto ahead) __attribute__((always_inline)) {
+    constexpr int kAhead = decltype(ahead)::value;
+    for (int first = part; first < chunks; first += 16 * kAhead) {
+      float keep[kAhead], sum[kAhead];
+      f32x4 x[kAhead][kQuads];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = first + j * 16 < chunks ? first + j * 16 : chunks - 1;
-      keep[j] = first + j * 16 < chunks ? stats[2 * c] : -__builtin_inff();
-      sum[j] = stats[2 * c + 1];
+      for (int j = 0; j < kAhead; ++j) {
+        const int c = first + j * 16 < chunks ? first + j * 16 : chunks - 1;
+        keep[j] = stats[2 * c];
+        sum[j] = stats[2 * c + 1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i * 64 + quad * 4 < p.dim)
-          x[j][i] = *reinterpret_cast<const f32x4*>(p.parts + (at + c) * p.dim + i * 64 + quad * 4);
+        for (int i = 0; i < kQuads; ++i)
+          if (i * 64 + quad * 4 < p.dim)
+            x[j][i] = *reinterpret_cast<const f32x4*>(p.parts + (at + c) * p.dim + i * 64 + quad * 4);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (first + j * 16 >= chunks) break;
+        const float weight = __builtin_amdgcn_exp2f(keep[j] - m_use);
+        l = __builtin_fmaf(sum[j], weight, l);
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+          if (i * 64 + quad * 4 < p.dim) o[i] += x[j][i] * weight;
+      }
     }
+  };
+  if (chunks > 16)
+    add(std::integral_constant<int, D == 256 ? 2 : 4>{});
+  else
+    add(std::integral_constant<int, 1>{});
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (first + j * 16 >= chunks) break;
-      const float weight = __builtin_amdgcn_exp2f(keep[j] - m_use);
-      l = __builtin_fmaf(sum[j], weight, l);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i * 64 + quad * 4 < p.dim) o[i] += x[j][i] * weight;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(sums[part][i * 16 + quad]) = o[i];
-  if (quad == 0) sums[part][64][0] = l;
+  for (int i = 0; i < kQuads; ++i) *reinterpret_cast<f32x4*>(sums[part][i * 16 + quad]) = o[i];
+  if (quad == 0) sums[part][D / 4][0] = l;
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= p.dim) return;
@@ -414,7 +425,7 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     total += sums[i][d / 4][d % 4];
-    l_all += sums[i][64][0];
+    l_all += sums[i][D / 4][0];
   }
   reinterpret_cast<T*>(p.out + b * p.out_row + head * p.out_head)[d] =
       (T)(m == -__builtin_inff() ? 0.f : total / l_all);
@@ -427,7 +438,7 @@ int launch_paged(const PagedParams& p, hipStream_t stream) {
                      dim3(64 * kWaves), 0, stream, p);
   OMNI_LAUNCH_CHECK();
   if (p.chunks > 1) {
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(p.batch * p.kv_heads * p.group)), dim3(256), 0,
+    hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(p.batch * p.kv_heads * p.group)), dim3(256), 0,
                        stream, p);
     OMNI_LAUNCH_CHECK();
   }
