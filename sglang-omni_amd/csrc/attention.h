@@ -69,8 +69,9 @@ OMNI_DEVICE float half_sum(float v) {
 // 64 pieces of 16 bytes, a lane's at base + off, into shared memory from `to` on, in the lanes' order; an
 // offset past the buffer's bytes gives zeros. Written out because the compiler, which knows of its own
 // such loads, waits for all of them before every transposed read, also where they fill another tile:
-// nothing but the caller's s_waitcnt vmcnt waits for these. (M0 holds the address, and takes a wait
-// state; nothing else in these kernels uses it.)
+// nothing but the caller's s_waitcnt vmcnt waits for these. M0 holds the address, and nothing else in these
+// kernels uses it. The wait states, which the compiler does not add here: one after M0, five where a vector
+// instruction (a readfirstlane, a spilled scalar's return) has just written the buffer's registers.
 OMNI_DEVICE u32x4 dma_rsrc(const uint8_t* base, uint32_t bytes) {
   const uint64_t at = (uint64_t)base;
   return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
@@ -78,7 +79,7 @@ OMNI_DEVICE u32x4 dma_rsrc(const uint8_t* base, uint32_t bytes) {
                (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 OMNI_DEVICE void dma_rows(u32x4 rsrc, uint32_t to, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane((int)to)), "v"(off), "s"(rsrc)
                : "memory");

@@ -184,6 +184,13 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
         q[s] = typename O::x8{};
     }
   }
+  // The queries, waited for here with the first tile: in its loop the compiler would wait for them again, and
+  // with them for the tile on its way. (Heads of 256 keep them where this would move them from; a chain of
+  // the other form is as long either way.)
+  if constexpr (LONG && D < 256) {
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) asm volatile("" : "+v"(q[s]));
+  }
   f32x16 o[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -287,6 +294,14 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
     for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * unit);
     *reinterpret_cast<typename O::x4*>(p.out + token * p.out_token + at_head * p.out_head + d * 2) = y;
   };
+  // The outputs through the matrix cores' pipeline: for code whose paths part and meet right after a product.
+  // Where such a meeting is reached straight and by a loop, the compiler counts the wait states before it
+  // along the longer way alone, and its copies there read results that are not there yet.
+  auto settle = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 3");
+    __builtin_amdgcn_sched_barrier(0);
+  };
   // what a row does not see: its scores
   auto hide = [&](int first_key, f32x16 (&s)[kBlocks]) __attribute__((always_inline)) {
 #pragma unroll
@@ -318,10 +333,12 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) zeros = O::mfma32(v_operand(stage, c, d), typename O::x8{}, zeros);
-      if (any(zeros))
+      if (any(zeros)) {
         bad = (1u << kSteps) - 1;
-      else
+      } else {
         accumulate(stage, w);
+        settle();
+      }
     } else {
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
@@ -342,6 +359,7 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
         }
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) o[d] = O::mfma32(v[d], w[c], o[d]);
+        settle();
       }
     }
     if (bad == 0) return;
@@ -351,9 +369,12 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
       const int c = e / 16, key = first_key + c * 16 + (e % 8 / 4) * 8 + (e % 16 / 8) * 4 + e % 4;
       if ((bad >> c & 1) == 0) continue;
       const bool mine = half == e % 16 / 8;
-      typename O::x8 wc = w[0];
+      // w[c], by masks: a choice by index would keep w in memory, on every call's way here
+      u32x4 bits = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int i = 1; i < kSteps; ++i) wc = c == i ? w[i] : wc;
+      for (int i = 0; i < kSteps; ++i)
+        bits |= __builtin_bit_cast(u32x4, w[i]) & (c == i ? 0xffffffffu : 0u);
+      const typename O::x8 wc = __builtin_bit_cast(typename O::x8, bits);
       typename O::x8 we;
 #pragma unroll
       for (int j = 0; j < 8; ++j) we[j] = mine && j == e % 8 ? wc[j] : (T)0.f;
@@ -388,10 +409,12 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
       scores_of(stage, s);
       if (partial) hide(first_key, s);
       weights_of(s, w);
-      if (partial)
+      if (partial) {
         accumulate_seen(first_key, stage, w);
-      else
+      } else {
         accumulate(stage, w);
+        settle();
+      }
     }
     // then whole tiles, the stage a constant of the code
     auto step = [&](int stage) __attribute__((always_inline)) {

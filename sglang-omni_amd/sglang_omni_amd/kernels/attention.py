@@ -55,7 +55,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     matrix cores take them; all sums are float32 and the output is rounded once. How a row's keys are
     divided over the chip follows from the call's sizes, and with it the row's last bits.
 
-    bf16 or f16; dim a multiple of 8 up to 256; heads contiguous and 16-byte aligned, other strides free.
+    bf16 or f16; dim a multiple of 8 up to 256; heads contiguous and 16-byte aligned, other strides free (of
+    k and v up to 2^23 between tokens); tokens * (heads // kv_heads) and key_tokens below 2^31 - 255.
     Rows of ``out`` behind the last sequence stay as they are; those of an output made here are zero."""
     index = q.get_device()
     if index < 0 or k.get_device() != index or v.get_device() != index:
