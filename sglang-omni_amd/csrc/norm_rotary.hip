@@ -81,7 +81,8 @@ OMNI_DEVICE void store_bytes(uint8_t* dst, int valid, const float (&v)[V], float
 //
 // WHOLE: every run of a chunk lies in the head. Then a lane's loads, of rows, weights, position and
 // frequencies, have no branch around them and go out at once (a load under a branch is waited for before
-// the next one goes out); lanes past the last chunk load it too and count nothing.
+// the next one goes out); lanes past the last chunk load it too, are not turned, and count nothing: neither
+// in the sum of squares nor in an 8-bit row's largest magnitude.
 template <typename T, int V, int ITERS, int HP, bool WHOLE>
 __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
   const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> p.lane_shift;
@@ -250,9 +251,12 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsParams p) {
     if (p.held == OMNI_DTYPE_FP8_E4M3) {
       float amax = 0.f;
 #pragma unroll
-      for (int t = 0; t < ITERS; ++t)
+      for (int t = 0; t < ITERS; ++t) {
+        float part = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) amax = fmaxf(amax, fmaxf(fabsf(a[i][t][v]), fabsf(b[i][t][v])));
+        for (int v = 0; v < V; ++v) part = fmaxf(part, fmaxf(fabsf(a[i][t][v]), fabsf(b[i][t][v])));
+        amax = fmaxf(amax, WHOLE && valid0[t] == 0 ? 0.f : part);
+      }
       for (int off = 1; off < lanes; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
       const float scale = group_scale(amax, &unit);
       if (lane == 0)
