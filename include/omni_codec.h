@@ -1063,8 +1063,9 @@ int omni_prompt_attention(const omni_prompt_args* args, omni_stream_t stream);
  * omni_paged_attention: one query of each sequence, q and out [batch][heads][dim] (bf16 or f16), over
  * the first lengths[b] (int32 / int64) keys of its cache: key j lies on page table[b][j / page_size]
  * (int32, rows table_stride apart), place j % page_size. The cache holds q's type or E4M3. Lengths count
- * up to the table's table_columns pages and to max_length; a negative one is 0, and a sequence without
- * keys is zero. Keys on pages outside [0, pages) are left out. Everything float32 but the products'
+ * up to the table's table_columns pages and to max_length; a negative one is 0. A sequence without keys is
+ * zero, and so is a row whose scores are all -infinity; a NaN among the scores makes the row NaN. Keys on
+ * pages outside [0, pages) are left out. Everything float32 but the products'
  * operands; outputs rounded once. A row's bits depend on its own sequence alone.
  *
  * Strides of q and out in elements, multiples of 8, pointers and the cache's rows 16-byte aligned; dim a

@@ -350,10 +350,11 @@ __global__ void __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) paged_kernel(co
         to[1] = l_all;
       }
     } else {
-      const float unit = m_all == -__builtin_inff() ? 0.f : 1.f / l_all;
+      // Zero by the sum, not by the maximum: that is -infinity where all scores are NaN, too.
+      const float unit = 1.f / l_all;
       typename O::x4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * unit);
+      for (int e = 0; e < 4; ++e) y[e] = (T)(l_all == 0.f ? 0.f : x[e] * unit);
       *reinterpret_cast<typename O::x4*>(p.out + b * p.out_row + out_head * p.out_head + d * 2) = y;
     }
   }
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p) {
     l_all += sums[i][D / 4][0];
   }
   reinterpret_cast<T*>(p.out + b * p.out_row + head * p.out_head)[d] =
-      (T)(m == -__builtin_inff() ? 0.f : total / l_all);
+      (T)(l_all == 0.f ? 0.f : total / l_all);
 }
 
 template <typename T, typename H, int D>

@@ -117,9 +117,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKvCache, table: torch.Tensor, l
     on them that the host knows (the table's room without it; longer ones count as it), and the closer it
     is the fewer idle workgroups and the less workspace a call takes.
 
-    A sequence without keys is zero; keys on pages outside the cache are left out. The cache holds q's
-    type (bf16 or f16) or E4M3, whose rows count their scale times the bytes; scale defaults to dim **
-    -0.5. A row's bits depend on its own sequence alone, not on the batch beside it nor on max_length."""
+    A sequence without keys is zero, and so is a row whose scores are all -infinity; a NaN among the scores
+    makes the row NaN. Keys on pages outside the cache are left out. The cache holds q's type (bf16 or f16)
+    or E4M3, whose rows count their scale times the bytes; scale defaults to dim ** -0.5. A row's bits depend on its own sequence alone, not on the batch beside it nor on max_length."""
     index = q.get_device()
     if index < 0 or cache.index != index or table.get_device() != index \
             or lengths.get_device() != index:
