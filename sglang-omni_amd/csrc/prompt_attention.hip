@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
   };
 
   // 4 dimensions of a row, from d on, out: the result, or where workgroups share the keys a part (without
-  // keys of its own its maximum alone)
+  // keys that count its maximum and sum alone). Which is which is told by the sum: zero where no score is
+  // above -infinity, NaN where one is NaN. The maximum is -infinity also where all are NaN.
   auto store_row = [&](int at_query, int at_head, int d, f32x4 x, float m, float l)
                        __attribute__((always_inline)) {
     const int64_t token = first + at_query;
@@ -285,13 +286,13 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
         stats[0] = m;
         stats[1] = l;
       }
-      if (m != -__builtin_inff()) *reinterpret_cast<f32x4*>(p.parts + at * p.dim + d) = x;
+      if (l != 0.f) *reinterpret_cast<f32x4*>(p.parts + at * p.dim + d) = x;
       return;
     }
-    const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
+    const float unit = 1.f / l;
     typename O::x4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * unit);
+    for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.f ? 0.f : x[e] * unit);
     *reinterpret_cast<typename O::x4*>(p.out + token * p.out_token + at_head * p.out_head + d * 2) = y;
   };
   // The outputs through the matrix cores' pipeline: for code whose paths part and meet right after a product.
@@ -515,7 +516,8 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
   }
   // A lane holds 4 dimensions of each 8; with the other half-wave's of one 8 for its own of the next it
   // stores 16 bytes at a time.
-  const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
+  const bool zero = l == 0.f;
+  const float unit = zero ? 0.f : 1.f / l;
   uint8_t* to = p.out + (int64_t)(first + query) * p.out_token + head * p.out_head;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -531,7 +533,8 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
       const auto r0 = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
       const auto r1 = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
       const int at = d * 32 + (i + half) * 8;
-      if (stored && at < p.dim) *reinterpret_cast<u32x4*>(to + at * 2) = u32x4{r0[0], r1[0], r0[1], r1[1]};
+      const u32x4 all = {r0[0], r1[0], r0[1], r1[1]}, none = {0u, 0u, 0u, 0u};  // none: the values may be NaN
+      if (stored && at < p.dim) *reinterpret_cast<u32x4*>(to + at * 2) = zero ? none : all;
     }
 }
 
@@ -554,15 +557,15 @@ __global__ void __launch_bounds__(256) join_kernel(const PromptParams p) {
   float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < p.splits; ++s) {
-    const float part = stats[(s * all + row) * 2];
-    if (part == -__builtin_inff()) continue;
-    const float keep = __builtin_amdgcn_exp2f(part - m);
-    l = __builtin_fmaf(stats[(s * all + row) * 2 + 1], keep, l);
+    const float sum = stats[(s * all + row) * 2 + 1];
+    if (sum == 0.f) continue;  // no part was stored
+    const float keep = __builtin_amdgcn_exp2f(stats[(s * all + row) * 2] - m);
+    l = __builtin_fmaf(sum, keep, l);
     const f32x4 x = *reinterpret_cast<const f32x4*>(p.parts + (s * all + row) * p.dim + d);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], keep, o[e]);
   }
-  const float unit = m == -__builtin_inff() ? 0.f : 1.f / l;
+  const float unit = l == 0.f ? 0.f : 1.f / l;
   typename Op<T>::x4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * unit);

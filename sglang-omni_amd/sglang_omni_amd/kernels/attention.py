@@ -50,8 +50,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
 
     Causal: a sequence's last query sees all of its keys, each one before it one key less, so the queries
     may be the last piece of a longer sequence. A query that sees no key (or whose scores are all
-    -infinity) is zero, and what lies behind a query's keys does not reach it, not even as NaN. scale
-    defaults to dim ** -0.5. Softmax weights are rounded to the type before they meet the values, as the
+    -infinity) is zero, one that sees a NaN score is NaN, and what lies behind a query's keys does not
+    reach it, not even as NaN. scale defaults to dim ** -0.5. Softmax weights are rounded to the type before they meet the values, as the
     matrix cores take them; all sums are float32 and the output is rounded once. How a row's keys are
     divided over the chip follows from the call's sizes, and with it the row's last bits.
 
