@@ -1022,10 +1022,11 @@ int omni_read_cache(const omni_read_cache_args* args, omni_stream_t stream);
  * clamped to [0, tokens] and [0, key_tokens]); query head h reads key head h / (heads / kv_heads).
  * Causal: the last query sees all of its sequence's keys, each one before it one key less. A query that
  * sees none, or whose scores are all -infinity, is zero; one that sees a NaN score is NaN; values behind
- * what a query sees do not reach it, whatever they hold. Rows of out outside the sequences stay as they are; with clear_rest those
- * from starts[sequences] on become zero. Scores, maxima and sums float32, softmax weights rounded to the
- * type before they meet the values, outputs rounded once. How the keys of a row are divided over waves
- * and workgroups follows from the call's sizes, so the last bits of a row may depend on what else is in it.
+ * what a query sees do not reach it, whatever they hold. Rows of out outside the sequences stay as they
+ * are; with clear_rest those in front of starts[0] and from starts[sequences] on become zero. Scores,
+ * maxima and sums float32, softmax weights rounded to the type before they meet the values, outputs
+ * rounded once. How the keys of a row are divided over waves and workgroups follows from the call's sizes,
+ * so the last bits of a row may depend on what else is in it.
  *
  * Strides in elements, multiples of 8, at most 2^23 between tokens of k and v; pointers 16-byte aligned;
  * dim a multiple of 8 up to 256; tokens * heads / kv_heads and key_tokens below 2^31 - 255; scale positive;

@@ -35,8 +35,8 @@ struct PromptParams {
   const void* key_starts;
   int wide;  // the starts are int64
   int tokens, key_tokens;  // tokens * group below 2^31
-  int sequences;  // and one past them where the rows behind the last one are cleared
-  int cleared;
+  int sequences;
+  int cleared;  // the rows in front of the first sequence and behind the last one become zero
   int kv_heads, group, dim, causal;
   float scale;  // of the scores, times log2(e)
   int slots;    // row tiles a key head, an upper bound
@@ -89,18 +89,19 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : D == 128 ? 2 : 1) promp
   const int slot = blockIdx.x / p.kv_heads / p.splits;
   // Sequence s owns the tiles from floor(first row / kRows) + s on: never fewer than it needs, and
   // found by search without a sum over the sequences before it: 64 at a time, each lane one's bounds.
-  int lo = 0, n = p.sequences;
+  // Rows that are cleared are two more sequences, the first and the last, without keys.
+  int lo = 0, n = p.sequences + 2 * p.cleared;
   int first, last, key_first, key_last;
   for (;;) {
     const int step = (n + 63) / 64, at = lane * step;
     int f = 0, l = 0, kf = 0, kl = 0;
     if (at < n) {
-      const bool rest = p.cleared && lo + at == p.sequences - 1;  // the rows behind the last sequence
-      f = start_of(p.starts, p.wide, lo + at, p.tokens);
-      l = rest ? p.tokens : start_of(p.starts, p.wide, lo + at + 1, p.tokens);
-      if (!rest) {
-        kf = start_of(p.key_starts, p.wide, lo + at, p.key_tokens);
-        kl = start_of(p.key_starts, p.wide, lo + at + 1, p.key_tokens);
+      const int s = lo + at - p.cleared;  // -1: the rows in front, p.sequences: those behind
+      f = s < 0 ? 0 : start_of(p.starts, p.wide, s, p.tokens);
+      l = s == p.sequences ? p.tokens : start_of(p.starts, p.wide, s + 1, p.tokens);
+      if (s >= 0 && s < p.sequences) {
+        kf = start_of(p.key_starts, p.wide, s, p.key_tokens);
+        kl = start_of(p.key_starts, p.wide, s + 1, p.key_tokens);
       }
     }
     const bool before = at < n && f * p.group / kRows + lo + at <= slot;
@@ -548,8 +549,8 @@ __global__ void __launch_bounds__(256) join_kernel(const PromptParams p) {
   const int d = (int)(item - row * quads) * 4;
   if (row >= all) return;
   const int token = (int)(row / heads);
-  if (token < start_of(p.starts, p.wide, 0, p.tokens) ||
-      (!p.cleared && token >= start_of(p.starts, p.wide, p.sequences, p.tokens)))
+  if (!p.cleared && (token < start_of(p.starts, p.wide, 0, p.tokens) ||
+                     token >= start_of(p.starts, p.wide, p.sequences, p.tokens)))
     return;
   const float* stats = p.parts + p.splits * all * p.dim;
   float m = -__builtin_inff();
@@ -577,7 +578,7 @@ template <typename T, int D, int NW, bool LONG>
 int launch_prompt(PromptParams p, hipStream_t stream) {
   constexpr int kTiles = 2 * keys_of(D, LONG) * D * 2;
   constexpr int kLds = LONG ? 2 * kTiles : NW * (kTiles + 64 * 4);
-  const int64_t slots = (int64_t)p.tokens * p.group / (LONG ? 32 * NW : 32) + p.sequences;
+  const int64_t slots = (int64_t)p.tokens * p.group / (LONG ? 32 * NW : 32) + p.sequences + 2 * p.cleared;
   if (slots * p.kv_heads * p.splits > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
   p.slots = (int)slots;
   if (kLds > 64 * 1024) {
@@ -703,7 +704,7 @@ extern "C" int omni_prompt_attention(const omni_prompt_args* a, omni_stream_t st
   p.tokens = (int)a->tokens;
   p.key_tokens = (int)a->key_tokens;
   p.cleared = a->clear_rest ? 1 : 0;
-  p.sequences = (int)a->sequences + p.cleared;
+  p.sequences = (int)a->sequences;
   p.kv_heads = (int)a->kv_heads;
   p.group = (int)(a->heads / a->kv_heads);
   p.dim = (int)a->dim;

@@ -45,8 +45,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     """softmax(scale q k^T) v of packed sequences, on the current stream: sequence s has the queries
     starts[s] .. starts[s + 1] - 1 of q [tokens, heads, dim] and the keys key_starts[s] .. key_starts[s +
     1] - 1 (starts without it) of k and v [key_tokens, kv_heads, dim]; query head h reads key head h //
-    (heads // kv_heads). Starts are int32 / int64 in device memory, from 0, ascending; the host does not
-    read them.
+    (heads // kv_heads). Starts are int32 / int64 in device memory, ascending; the host does not read
+    them.
 
     Causal: a sequence's last query sees all of its keys, each one before it one key less, so the queries
     may be the last piece of a longer sequence. A query that sees no key (or whose scores are all
@@ -57,7 +57,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
 
     bf16 or f16; dim a multiple of 8 up to 256; heads contiguous and 16-byte aligned, other strides free (of
     k and v up to 2^23 between tokens); tokens * (heads // kv_heads) and key_tokens below 2^31 - 255.
-    Rows of ``out`` behind the last sequence stay as they are; those of an output made here are zero."""
+    Rows of ``out`` in front of the first sequence and behind the last one stay as they are; those of an
+    output made here are zero."""
     index = q.get_device()
     if index < 0 or k.get_device() != index or v.get_device() != index:
         N.require_device(q, k, v)
