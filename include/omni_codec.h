@@ -962,8 +962,8 @@ typedef struct omni_kv_cache {
  *
  * float32 throughout, rounded once to the type; the cache gets the rounded values. heads may be 0, and
  * k_out null where only the cache takes k; v is read with a cache only. q_out may be q and k_out k
- * (same strides), else nothing overlaps. dim up to 512 (else OMNI_ERR_UNSUPPORTED); tokens = 0 does
- * nothing.
+ * (same strides), else nothing overlaps. dim up to 512, and no more rows than a launch of 2^32 - 1 threads
+ * takes (else OMNI_ERR_UNSUPPORTED, here and below); tokens = 0 does nothing.
  */
 typedef struct omni_norm_rotary_args {
   const void* q;

@@ -10,6 +10,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
+// Workgroups of 256 threads that a launch can have: a grid's threads count in 32 bits.
+constexpr int64_t kMostWorkgroups = 0xffffff;
+
 // A cache as the kernels take it: rows [pages][kv_heads][page_size][dim], strides in elements (all
 // below 2^31 rows, so slots are 32-bit).
 struct CacheView {

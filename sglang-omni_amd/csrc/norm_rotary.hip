@@ -285,7 +285,7 @@ int launch_heads(HeadsParams p, int64_t tokens, hipStream_t stream) {
   for (int kind = 0; kind < 3; ++kind) p.groups[kind] = (p.heads[kind] + HP - 1) / HP;
   p.items = tokens * (p.groups[0] + p.groups[1] + p.groups[2]);
   const int64_t workgroups = ((p.items << p.lane_shift) + 255) / 256;
-  if (workgroups > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+  if (workgroups > kMostWorkgroups) return OMNI_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((heads_kernel<T, V, ITERS, HP, WHOLE>), dim3((unsigned)workgroups), dim3(256), 0, stream, p);
   OMNI_LAUNCH_CHECK();
   return OMNI_OK;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadParams p) {
 template <typename H, typename T>
 int launch_read(const ReadParams& p, hipStream_t stream) {
   const int64_t workgroups = (p.items + 255) / 256;
-  if (workgroups > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+  if (workgroups > kMostWorkgroups) return OMNI_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((read_kernel<H, T>), dim3((unsigned)workgroups), dim3(256), 0, stream, p);
   OMNI_LAUNCH_CHECK();
   return OMNI_OK;

@@ -495,8 +495,9 @@ extern "C" int omni_paged_attention(const omni_paged_args* a, omni_stream_t stre
     return OMNI_ERR_INVALID_ARG;
   const int64_t kv_heads = a->cache->kv_heads, group = a->heads / kv_heads;
   const int64_t tiles = (group + 15) / 16;
-  if (kv_heads * tiles > 65535 || a->batch * a->heads > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+  if (kv_heads * tiles > 65535) return OMNI_ERR_UNSUPPORTED;
   const int64_t chunks = most_chunks(a->max_length, (int)kv_heads, (int)tiles);
+  if (chunks > 1 && a->batch * a->heads > kMostWorkgroups) return OMNI_ERR_UNSUPPORTED;
   if (chunks > 1 && (!a->workspace || !aligned_to(a->workspace, 16) ||
                      a->workspace_bytes < a->batch * a->heads * chunks * (a->cache->dim + 2) * 4))
     return OMNI_ERR_INVALID_ARG;

@@ -579,7 +579,9 @@ int launch_prompt(PromptParams p, hipStream_t stream) {
   constexpr int kTiles = 2 * keys_of(D, LONG) * D * 2;
   constexpr int kLds = LONG ? 2 * kTiles : NW * (kTiles + 64 * 4);
   const int64_t slots = (int64_t)p.tokens * p.group / (LONG ? 32 * NW : 32) + p.sequences + 2 * p.cleared;
-  if (slots * p.kv_heads * p.splits > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
+  const int64_t quads = (int64_t)p.tokens * p.kv_heads * p.group * (p.dim / 4);
+  const int64_t joins = p.splits > 1 ? (quads + 255) / 256 : 0;
+  if (slots * p.kv_heads * p.splits > kMostWorkgroups || joins > kMostWorkgroups) return OMNI_ERR_UNSUPPORTED;
   p.slots = (int)slots;
   if (kLds > 64 * 1024) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, D, NW, LONG>),
@@ -589,10 +591,8 @@ int launch_prompt(PromptParams p, hipStream_t stream) {
   hipLaunchKernelGGL((prompt_kernel<T, D, NW, LONG>), dim3((unsigned)(slots * p.kv_heads * p.splits)),
                      dim3(64 * NW), kLds, stream, p);
   OMNI_LAUNCH_CHECK();
-  if (p.splits > 1) {
-    const int64_t items = (int64_t)p.tokens * p.kv_heads * p.group * (p.dim / 4);
-    if ((items + 255) / 256 > 0x7fffffffLL) return OMNI_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, p);
+  if (joins > 0) {
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)joins), dim3(256), 0, stream, p);
     OMNI_LAUNCH_CHECK();
   }
   return OMNI_OK;
