@@ -39,7 +39,6 @@ struct PromptParams {
   int cleared;  // the rows in front of the first sequence and behind the last one become zero
   int kv_heads, group, dim, causal;
   float scale;  // of the scores, times log2(e)
-  int slots;    // row tiles a key head, an upper bound
   int splits;   // workgroups that share a row tile's keys
   float* parts;  // with several: [splits][tokens][heads][dim], then [splits][tokens][heads][2] of m and l
 };
@@ -64,7 +63,6 @@ OMNI_DEVICE int v_slot(int r, int p) {
   return D == 64 ? p ^ (((r >> 1) & 1) * 4) : p ^ ((r & 3) * 4);
 }
 
-//
 // LONG: the waves own 32 rows each and share the tiles, [2][K, V] in shared memory, the next one on its
 // way. Not LONG, for few rows: the waves share 32 rows and each owns every NW-th tile, [NW][K, V], and
 // their parts are joined at the end; so many more workgroups, each with fewer tiles one after the other.
@@ -582,7 +580,6 @@ int launch_prompt(PromptParams p, hipStream_t stream) {
   const int64_t quads = (int64_t)p.tokens * p.kv_heads * p.group * (p.dim / 4);
   const int64_t joins = p.splits > 1 ? (quads + 255) / 256 : 0;
   if (slots * p.kv_heads * p.splits > kMostWorkgroups || joins > kMostWorkgroups) return OMNI_ERR_UNSUPPORTED;
-  p.slots = (int)slots;
   if (kLds > 64 * 1024) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, D, NW, LONG>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
