@@ -97,16 +97,23 @@ class ContextTalker:
                  for q in range(c.codebooks)]
         self.allowed = torch.stack(masks).to(torch.int32).to(device)
 
-    def grow(self, stream: int, tokens: int) -> list[int]:
-        """Room for `tokens` more tokens of a stream: their slots."""
-        c, pages, length = self.config, self.pages[stream], self.lengths[stream]
-        while len(pages) * c.page_size < length + tokens:
-            if not self.free:
-                raise RuntimeError("no free page")
-            pages.append(self.free.pop())
-            self.table[stream, len(pages) - 1] = pages[-1]
-        self.lengths[stream] += tokens
-        return self.slots(stream, length, length + tokens)
+    def grow(self, streams: list[int], tokens: list[int]) -> list[int]:
+        """Room for so many more tokens of each stream, of all of them or of none: their slots."""
+        c = self.config
+        if len(set(streams)) != len(streams) or min(tokens) < 1:
+            raise ValueError("a call takes one token or more of each of its streams, each once")
+        wanted = [-(-(self.lengths[s] + n) // c.page_size) - len(self.pages[s])
+                  for s, n in zip(streams, tokens)]
+        if sum(wanted) > len(self.free):
+            raise RuntimeError("no free page")
+        slots = []
+        for s, n, more in zip(streams, tokens, wanted):
+            for _ in range(more):
+                self.pages[s].append(self.free.pop())
+                self.table[s, len(self.pages[s]) - 1] = self.pages[s][-1]
+            slots += self.slots(s, self.lengths[s], self.lengths[s] + n)
+            self.lengths[s] += n
+        return slots
 
     def slots(self, stream: int, start: int, end: int) -> list[int]:
         size = self.config.page_size
@@ -146,7 +153,7 @@ class ContextTalker:
         after each stream's last one."""
         device = self.embedding.device
         before = [self.lengths[s] for s in streams]
-        slots = [slot for s, t in zip(streams, tokens) for slot in self.grow(s, len(t))]
+        slots = self.grow(streams, [len(t) for t in tokens])
         ends = torch.tensor([len(t) for t in tokens]).cumsum(0)
         starts = torch.cat([ends.new_zeros(1), ends]).to(device)
         positions = torch.tensor([b + i for b, t in zip(before, tokens) for i in range(len(t))],
@@ -171,7 +178,7 @@ class ContextTalker:
         """One more token of each stream: the logits after it."""
         device = self.embedding.device
         positions = torch.tensor([self.lengths[s] for s in streams], device=device)
-        slots = torch.tensor([self.grow(s, 1)[0] for s in streams], device=device)
+        slots = torch.tensor(self.grow(streams, [1] * len(streams)), device=device)
         longest = max(self.lengths[s] for s in streams)
         table = self.table[streams]
 
