@@ -6,18 +6,20 @@
 // A sequence without keys is zero. Keys on a page outside the cache are left out.
 //
 // The cache is read once, and that bounds it: 2 x 131072 keys of 8 heads of 128 in 100 us in 8 bits (5.5
-// TB/s; a plain read of 1 GiB 6.3, a copy 5.06) and 183 in bf16 (5.9), 64 streams up to 5000 in 148 (4.95);
-// one stream of 300 in 7.7, a chain of loads: length, table, rows. A sequence's keys are cut into chunks whose size follows
-// from its length alone, so that a row's bits do not depend on the batch; a workgroup takes a chunk of a
-// key head for up to 16 query heads, its four waves every fourth tile of 32 keys each, with their own
-// running maximum and sum, joined through shared memory. One chunk is the result; several are joined by
-// a second launch, in their order.
+// TB/s; a plain read of 1 GiB 6.3, a copy 5.06) and 187 in bf16 (5.7), 64 streams up to 5000 in 139 - 143
+// (5.1 - 5.3); one stream of 300 in 7.6, a chain of loads: length, table, rows. (In a graph, as below.) A
+// sequence's keys are cut into chunks whose size follows from its length alone, so that a row's bits do not
+// depend on the batch; a workgroup takes a chunk of a key head for up to 16 query heads, its four waves every
+// fourth tile of 32 keys each, with their own running maximum and sum, joined through shared memory. One
+// chunk is the result; several are joined by a second launch, in their order.
 //
 // Scores transposed, S^T = K Q^T (16 x 16 x 32 MFMAs, K's rows from memory straight into operands: the
 // dimensions of a row in any order, so long as q's are in the same), and O^T = V^T P^T as in the prompt
 // kernel, V read transposed from shared memory. bf16 weights are held as a sum of two bf16 numbers, 16
-// bits of each weight: the matrix cores have nothing else to do here. 8-bit rows widen exactly; the keys'
-// scales multiply the scores and the values' the weights.
+// bits of each weight: the matrix cores have nothing else to do here. float16 ones are one number: 11 bits,
+// as many as the result is rounded to (9 streams up to 20000: 2.3e-4 from float64 in the mean square, the
+// rounding alone 2.0e-4). 8-bit rows widen exactly; the keys' scales multiply the scores and the values'
+// the weights.
 #include <initializer_list>
 #include <type_traits>
 

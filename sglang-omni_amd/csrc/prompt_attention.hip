@@ -16,7 +16,7 @@
 // unrounded ones); scores, maxima, sums and outputs are float32.
 //
 // The matrix cores bound long prompts, and the clock that falls under them: 16384 tokens of 32 heads over 8
-// of 128, causal, 1966 - 2097 us, 1049 - 1118 TFLOP/s (a library's 8192^3 product 1237). Per 64 keys a wave
+// of 128, causal, 1950 - 2010 us, 1094 - 1128 TFLOP/s (a library's 8192^3 product 1237). Per 64 keys a wave
 // has 1024 cycles of MFMAs and about 670 of the softmax's, which another wave's MFMAs hide. Short ones are
 // latency: 37 tokens 7 us, bounds, then keys and queries, a tile or two, the join.
 #include <type_traits>
